@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-from .build import LIB, LIB_REFINE
+from .build import LIB, LIB_FFN, LIB_REFINE
 
 # Status codes (include/bvml_dsine.h)
 OK = 0
@@ -73,8 +73,32 @@ EWEIGHTS = -9
 EFILE = -10
 ELIB = -11
 
+
+# Every symbol include/bvml_ffn.h declares.
+FFN_EXPORTS = (
+    "bvml_ffn_add_rms_norm",
+    "bvml_ffn_add_rms_norm_backward",
+    "bvml_ffn_add_rms_norm_backward_workspace",
+    "bvml_ffn_linear",
+    "bvml_ffn_linear_workspace",
+    "bvml_ffn_linear_backward",
+    "bvml_ffn_linear_backward_workspace",
+    "bvml_ffn_gated",
+    "bvml_ffn_gated_workspace",
+    "bvml_ffn_gated_backward",
+    "bvml_ffn_gated_backward_workspace",
+    "bvml_ffn_plan",
+    "bvml_ffn_last_error",
+    "bvml_ffn_version",
+)
+# Status codes, element types and activations (include/bvml_ffn.h)
+FFN_ENULL, FFN_ESHAPE, FFN_ETYPE, FFN_ESIZE, FFN_EALIAS, FFN_EPARAM, FFN_EWORK = range(-1, -8, -1)
+F32, F16, BF16, E4M3 = range(4)
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
 _lib = None
 _refine = None
+_ffn = None
 
 
 def load(path: str = LIB) -> ctypes.CDLL:
@@ -189,6 +213,68 @@ def load_refine(path: str = LIB_REFINE) -> ctypes.CDLL:
     lib.bvml_dsine_refiner_last_error.restype = ctypes.c_char_p
     _refine = lib
     return lib
+
+
+def load_ffn(path: str = LIB_FFN) -> ctypes.CDLL:
+    """Load (once) and type the feed-forward library (include/bvml_ffn.h);
+    raises if it was not built."""
+    global _ffn
+    if _ffn is not None:
+        return _ffn
+    if not os.path.exists(path):
+        raise RuntimeError(
+            f"brovisionml_amd: native library {path} is missing; run "
+            "`python -m brovisionml_amd.build` (hipcc, gfx950) first")
+    lib = ctypes.CDLL(path)
+    vp, i, ll, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
+    ip = ctypes.POINTER(ctypes.c_int)
+    lib.bvml_ffn_add_rms_norm.argtypes = [vp, ll, vp, ll, vp, i, i, d, i, i, i, vp, ll, vp, ll, vp,
+                                          vp, vp]
+    lib.bvml_ffn_add_rms_norm_backward.argtypes = [vp, ll, vp, ll, vp, vp, vp, ll, i, i, i, i, i,
+                                                   vp, ll, vp, vp, ll, vp]
+    lib.bvml_ffn_linear.argtypes = [vp, ll, vp, ll, vp, vp, vp, vp, ll, i, i, i, i, i, i, i, vp, ll,
+                                    vp, ll, vp, ll, vp]
+    lib.bvml_ffn_gated.argtypes = [vp, ll, vp, ll, vp, vp, vp, i, i, i, i, i, i, i, vp, ll, vp, ll,
+                                   vp, ll, vp]
+    for name in ("bvml_ffn_linear_backward", "bvml_ffn_gated_backward"):
+        getattr(lib, name).argtypes = [vp, ll, vp, ll, vp, ll, vp, ll, i, i, i, i, i, i, vp, ll, vp,
+                                       ll, vp, vp, ll, vp]
+    lib.bvml_ffn_plan.argtypes = [i, i, i, i, i, i, i, ip, ip, ip]
+    for name in ("bvml_ffn_add_rms_norm", "bvml_ffn_add_rms_norm_backward", "bvml_ffn_linear",
+                 "bvml_ffn_gated", "bvml_ffn_linear_backward", "bvml_ffn_gated_backward",
+                 "bvml_ffn_plan"):
+        getattr(lib, name).restype = i
+    lib.bvml_ffn_add_rms_norm_backward_workspace.argtypes = [i, i]
+    for name in ("bvml_ffn_linear_workspace", "bvml_ffn_gated_workspace"):
+        getattr(lib, name).argtypes = [i, i, i, i]
+    for name in ("bvml_ffn_linear_backward_workspace", "bvml_ffn_gated_backward_workspace"):
+        getattr(lib, name).argtypes = [i, i, i]
+    for name in ("bvml_ffn_add_rms_norm_backward_workspace", "bvml_ffn_linear_workspace",
+                 "bvml_ffn_gated_workspace", "bvml_ffn_linear_backward_workspace",
+                 "bvml_ffn_gated_backward_workspace"):
+        getattr(lib, name).restype = ll
+    for name in ("bvml_ffn_last_error", "bvml_ffn_version"):
+        getattr(lib, name).argtypes = []
+        getattr(lib, name).restype = ctypes.c_char_p
+    _ffn = lib
+    return lib
+
+
+def ffn_last_error() -> str:
+    return load_ffn().bvml_ffn_last_error().decode()
+
+
+def ffn_plan(M: int, R: int, K: int, in_type: int, layout: int = 0, gated: bool = False,
+             aligned: bool = True):
+    """(rows of a tile (0: the few-rows kernel), operands straight to LDS?,
+    parts of the sum) of a product of C (M, R) over K; raises on a rejected
+    argument."""
+    tile, dma, splits = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    st = load_ffn().bvml_ffn_plan(M, R, K, in_type, layout, int(gated), int(aligned),
+                                  ctypes.byref(tile), ctypes.byref(dma), ctypes.byref(splits))
+    if st != OK:
+        raise RuntimeError(f"ffn_plan: {ffn_last_error()} (status {st})")
+    return tile.value, bool(dma.value), splits.value
 
 
 def refine_last_error() -> str:

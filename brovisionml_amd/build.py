@@ -15,6 +15,9 @@
                           (dsine_refine.cpp, include/brovisionml/dsine_refine.h)
                           over the refiner's C ABI; brotensor::Tensor left
                           undefined, like libbvml_dsine_cxx.so
+  libbvml_ffn.so          the feed-forward operators (include/bvml_ffn.h): HIP
+                          kernels behind a C ABI of their own; extern "C"
+                          symbols only
   libbrotensor_subset.so  the brotensor::Tensor subset of
                           include/brotensor/tensor.h, for standalone use and
                           the C++ tests; a brovisionml build links brotensor
@@ -25,6 +28,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "brovisionml_amd")
@@ -36,6 +40,7 @@ LIB_CXX = os.path.join(LIBDIR, "libbvml_dsine_cxx.so")
 LIB_TENSOR = os.path.join(LIBDIR, "libbrotensor_subset.so")
 LIB_REFINE = os.path.join(LIBDIR, "libbvml_dsine_refine.so")
 LIB_REFINE_CXX = os.path.join(LIBDIR, "libbvml_dsine_refine_cxx.so")
+LIB_FFN = os.path.join(LIBDIR, "libbvml_ffn.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -82,6 +87,11 @@ REFINE_SOURCES = [os.path.join(CSRC, "refiner.cpp"),      # device path, weights
 # scratch array (hipcc)
 REFINE_HIP_SOURCES = [os.path.join(CSRC, "refiner_conv.hip"),
                       os.path.join(CSRC, "refiner_noalloc.hip")]
+# the feed-forward operators: C entry points, the products (a translation unit
+# an operand type, compiled side by side), the norm, the activations' slopes
+FFN_SOURCES = [os.path.join(CSRC, name + ".hip") for name in (
+    "ffn_product_bf16", "ffn_product_f16", "ffn_product_e4m3", "ffn_product", "ffn_norm",
+    "ffn_slope", "ffn")]
 # host C++ against the HIP runtime headers
 HIP_HOST_FLAGS = ["-D__HIP_PLATFORM_AMD__", "-isystem", os.path.join(ROCM, "include")]
 
@@ -97,8 +107,20 @@ def _install(tmp: str, dst: str) -> None:
     os.replace(tmp, dst)
 
 
+def _build_ffn(objdir: str, status_obj: str) -> None:
+    def compile_one(src: str) -> str:
+        obj = os.path.join(objdir, os.path.basename(src) + ".o")
+        _run([HIPCC, *HIP_FLAGS, "-I", INCLUDE, "-c", src, "-o", obj])
+        return obj
+    with ThreadPoolExecutor(4) as pool:
+        objs = list(pool.map(compile_one, FFN_SOURCES))
+    _run([HIPCC, "--offload-arch=gfx950", "-shared", "-o", LIB_FFN + ".tmp", *objs, status_obj,
+          "-Wl,--version-script=" + os.path.join(CSRC, "libbvml_ffn.map")])
+    _install(LIB_FFN + ".tmp", LIB_FFN)
+
+
 def build_library() -> str:
-    """Builds the five libraries; returns the C ABI library's path."""
+    """Builds the six libraries; returns the DSINE ops' C ABI library's path."""
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(PKG, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -129,6 +151,7 @@ def build_library() -> str:
           "-L", LIBDIR, "-lbvml_dsine", "-Wl,-rpath,$ORIGIN",
           "-Wl,--version-script=" + os.path.join(CSRC, "libbvml_dsine_cxx.map")])
     _install(LIB_CXX + ".tmp", LIB_CXX)
+    _build_ffn(objdir, os.path.join(objdir, "status.cpp.o"))
     _run([HIPCC, "-O2", "-std=c++17", "-fPIC", "-I", INCLUDE, "-shared", "-o", LIB_TENSOR + ".tmp",
           *TENSOR_SOURCES])
     _install(LIB_TENSOR + ".tmp", LIB_TENSOR)

@@ -1,0 +1,245 @@
+// What the feed-forward kernels share: element types, vector loads and stores
+// of any alignment, the activations with their slopes, and the epilogue of a
+// product.  Private to libbvml_ffn.so.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "bvml_ffn.h"
+
+namespace bvml_ffn {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// Element types, as the C ABI numbers them.
+constexpr int kF32 = BVML_FFN_F32, kF16 = BVML_FFN_F16, kBF16 = BVML_FFN_BF16,
+              kE4M3 = BVML_FFN_E4M3;
+
+// ---------------------------------------------------------------------------
+// conversions: sums and statistics are fp32; every rounding to 16 bits goes
+// to nearest even, once, where a result is stored
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float from16(uint16_t bits, int type) {
+    return type == kBF16 ? __builtin_bit_cast(float, (uint32_t)bits << 16)
+                         : (float)__builtin_bit_cast(_Float16, bits);
+}
+__device__ __forceinline__ uint16_t to16(float v, int type) {
+    return type == kBF16 ? __builtin_bit_cast(uint16_t, (__bf16)v)
+                         : __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+// V consecutive values at element `at` of a 16- or 32-bit array, the first n
+// of them inside it (the others read as 0).  Whole vectors are one load of
+// up to 16 bytes at any alignment (the hardware takes unaligned global
+// accesses); only a row's ragged end goes value by value.
+template <int V>
+__device__ __forceinline__ void load_row(const void* base, int type, long long at, int n,
+                                         float (&v)[V]) {
+    if (type == kF32) {
+        const float* p = static_cast<const float*>(base) + at;
+        if (n >= V) {
+            __builtin_memcpy(v, p, 4 * V);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = i < n ? p[i] : 0.0f;
+        }
+        return;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    uint16_t h[V];
+    if (n >= V) {
+        __builtin_memcpy(h, p, 2 * V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[i] = i < n ? p[i] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = from16(h[i], type);
+}
+
+template <int V>
+__device__ __forceinline__ void store_row(void* base, int type, long long at, int n,
+                                          const float (&v)[V]) {
+    if (type == kF32) {
+        float* p = static_cast<float*>(base) + at;
+        if (n >= V) {
+            __builtin_memcpy(p, v, 4 * V);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i < n) p[i] = v[i];
+        }
+        return;
+    }
+    uint16_t h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = to16(v[i], type);
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    if (n >= V) {
+        __builtin_memcpy(p, h, 2 * V);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < n) p[i] = h[i];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// activations, in fp32 on the hardware's 2^x and reciprocal (about 1 ulp each)
+// ---------------------------------------------------------------------------
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float sigmoid_fast(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x));
+}
+
+// The normal distribution's Phi(x), with e = exp(-x^2 / 2): erfc by
+// Abramowitz and Stegun's formula 7.1.26, whose error is at most 1.5e-7, on
+// the side where it does not cancel.
+__device__ __forceinline__ float normal_cdf(float x, float e) {
+    const float a = __builtin_fabsf(x) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
+    const float p =
+        t * (0.254829592f +
+             t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float tail = 0.5f * p * e;
+    return x < 0.0f ? tail : 1.0f - tail;
+}
+
+// 0.5 (1 + tanh(a)) = sigmoid(2 a), a = sqrt(2 / pi) (x + 0.044715 x^3)
+constexpr float kTanhA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kTanhB = 0.044715f;
+
+__device__ __forceinline__ float act1(int act, float x) {
+    switch (act) {
+        case BVML_FFN_RELU: return x < 0.0f ? 0.0f : x;
+        case BVML_FFN_GELU: return x * normal_cdf(x, exp_fast(-0.5f * x * x));
+        case BVML_FFN_GELU_TANH: return x * sigmoid_fast(kTanhA * (x + kTanhB * x * x * x));
+        case BVML_FFN_SILU: return x * sigmoid_fast(x);
+        default: return x;
+    }
+}
+
+// The activation and its derivative.
+__device__ __forceinline__ void act_slope1(int act, float x, float& value, float& slope) {
+    switch (act) {
+        case BVML_FFN_RELU:
+            value = x < 0.0f ? 0.0f : x;
+            slope = x > 0.0f ? 1.0f : 0.0f;
+            return;
+        case BVML_FFN_GELU: {
+            const float e = exp_fast(-0.5f * x * x);
+            const float c = normal_cdf(x, e);
+            value = x * c;
+            slope = c + x * e * 0.3989422804014327f;
+            return;
+        }
+        case BVML_FFN_GELU_TANH: {
+            const float s = sigmoid_fast(kTanhA * (x + kTanhB * x * x * x));
+            value = x * s;
+            slope = s + x * s * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * x * x);
+            return;
+        }
+        case BVML_FFN_SILU: {
+            const float s = sigmoid_fast(x);
+            value = x * s;
+            slope = s + x * s * (1.0f - s);
+            return;
+        }
+        default:
+            value = x;
+            slope = 1.0f;
+    }
+}
+
+// `act` is the same for the whole launch: one scalar branch per vector
+template <int V>
+__device__ __forceinline__ void activate(int act, float (&v)[V]) {
+    switch (act) {
+#define BVML_FFN_CASE(A)                                    \
+    case A:                                                 \
+        _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = act1(A, v[i]); \
+        break;
+        BVML_FFN_CASE(BVML_FFN_RELU)
+        BVML_FFN_CASE(BVML_FFN_GELU)
+        BVML_FFN_CASE(BVML_FFN_GELU_TANH)
+        BVML_FFN_CASE(BVML_FFN_SILU)
+#undef BVML_FFN_CASE
+        default: break;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// a product's epilogue
+// ---------------------------------------------------------------------------
+struct Epilogue {
+    const void* bias;       // (R) of bias_type, or null
+    const float* x_scale;   // (M) with w_scale (R), or null
+    const float* w_scale;
+    const void* residual;   // (M, N) of out_type, or null
+    void* y;                // (M, N) of out_type
+    void* z;                // (M, R) of z_type: the pre-activations, or null
+    float* part;            // (splits, M, R) partial sums, or null
+    long long ldr, ldy, ldz;
+    int M, N;               // N: y's columns; R = N, or 2N for the gated form
+    int bias_type, out_type, z_type, act;
+};
+
+// V neighbouring sums of row m from column n on.
+template <int V>
+__device__ __forceinline__ void affine(const Epilogue& e, int m, int col, int c, float (&v)[V]) {
+    if (e.x_scale) {
+        const float s = e.x_scale[m];
+        float w[V];
+        load_row<V>(e.w_scale, kF32, col, c, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= s * w[i];
+    }
+    if (e.bias) {
+        float b[V];
+        load_row<V>(e.bias, e.bias_type, col, c, b);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] += b[i];
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void finish(const Epilogue& e, int m, int n, float (&v)[V]) {
+    const int c = e.N - n;
+    if (m >= e.M || c <= 0) return;
+    affine<V>(e, m, n, c, v);
+    if (e.z) store_row<V>(e.z, e.z_type, (long long)m * e.ldz + n, c, v);
+    activate<V>(e.act, v);
+    if (e.residual) {
+        float r[V];
+        load_row<V>(e.residual, e.out_type, (long long)m * e.ldr + n, c, r);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] += r[i];
+    }
+    store_row<V>(e.y, e.out_type, (long long)m * e.ldy + n, c, v);
+}
+
+// act(gate) * up for V neighbouring columns.
+template <int V>
+__device__ __forceinline__ void finish_gated(const Epilogue& e, int m, int n, float (&g)[V],
+                                             float (&u)[V]) {
+    const int c = e.N - n;
+    if (m >= e.M || c <= 0) return;
+    affine<V>(e, m, n, c, g);
+    affine<V>(e, m, e.N + n, c, u);
+    if (e.z) {
+        store_row<V>(e.z, e.z_type, (long long)m * e.ldz + n, c, g);
+        store_row<V>(e.z, e.z_type, (long long)m * e.ldz + e.N + n, c, u);
+    }
+    activate<V>(e.act, g);
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] *= u[i];
+    store_row<V>(e.y, e.out_type, (long long)m * e.ldy + n, c, g);
+}
+
+}  // namespace bvml_ffn

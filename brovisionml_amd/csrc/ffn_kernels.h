@@ -1,0 +1,100 @@
+// The feed-forward library's kernels as its C entry points call them.
+// Private to libbvml_ffn.so.
+#pragma once
+
+#include "ffn_common.h"
+
+namespace bvml_ffn {
+
+// Which operand lies with k across its rows (ffn_product.h).
+enum Layout { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
+
+// A product's operands and sums; its kernel, tile and split are chosen by
+// plan_product.
+struct ProductCall {
+    const void* p;
+    const void* q;
+    long long ldp, ldq;  // elements from row to row
+    int M, R, K;
+    int in_type;
+    int layout;
+    bool gated;
+    bool padded_p;  // P's rows end on 16 bytes, zeros from K (columns: from M) on
+    Epilogue e;
+};
+
+enum Tile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTileRows = 3 };
+
+struct ProductPlan {
+    int tile;    // a Tile; kTileRows: the few-rows kernel
+    bool dma;    // copies go straight to LDS
+    int splits;  // the sum's parts, joined by a second launch
+};
+
+// The kernel for a product of these sizes (dma: dma_fits of its operands).
+ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma);
+bool dma_fits(const ProductCall& c);
+// bytes of partial sums the plan needs, with and without direct copies
+long long product_workspace(int M, int R, int K, int in_type, int layout, bool gated);
+hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s);
+
+// One translation unit an element type (ffn_product_*.hip).
+struct Product;
+hipError_t launch_tiles_f16(const Product& a, const ProductPlan& p, int layout, bool gated,
+                            hipStream_t s);
+hipError_t launch_tiles_bf16(const Product& a, const ProductPlan& p, int layout, bool gated,
+                             hipStream_t s);
+hipError_t launch_tiles_e4m3(const Product& a, const ProductPlan& p, int layout, bool gated,
+                             hipStream_t s);
+struct NormCall {
+    const void* x;
+    const void* residual;
+    const void* weight;
+    long long ldx, ldr, ldy, lds;
+    int rows, cols;
+    float eps;
+    int x_type, w_type, y_type;
+    void* y;
+    void* stream_out;
+    float* scale;
+    float* rstd;
+};
+hipError_t launch_norm(const NormCall& c, hipStream_t s);
+
+struct NormGradCall {
+    const void* dy;
+    const void* stream_in;
+    const void* weight;
+    const float* rstd;
+    const void* dstream;
+    long long lddy, lds, ldds, lddx;
+    int rows, cols;
+    int dy_type, x_type, w_type;
+    void* dx;
+    void* dweight;
+    float* workspace;
+};
+long long norm_grad_workspace(int rows, int cols);
+hipError_t launch_norm_grad(const NormGradCall& c, hipStream_t s);
+
+// dz = dy act'(z) (linear) or [dy up act'(gate), dy act(gate)] (gated), in
+// 16 bits with rows of ldd elements (zeros beyond the last column), and the
+// sums of its columns.
+struct SlopeCall {
+    const void* dy;
+    const void* z;  // null: dz = dy
+    long long lddy, ldz, ldd;
+    int rows, N;
+    bool gated;
+    int dy_type, type, act;
+    void* dz;    // null: only the sums
+    void* db;    // null: only dz
+    float* workspace;
+};
+// out[c] = the sum of `parts` rows of cols floats
+hipError_t launch_column_sum(const float* part, int parts, int cols, void* out, int type,
+                             hipStream_t s);
+long long slope_workspace(int rows, int R);
+hipError_t launch_slope(const SlopeCall& c, hipStream_t s);
+
+}  // namespace bvml_ffn

@@ -1,0 +1,260 @@
+// RMS norm with the residual's addition, and its gradient.
+//
+// Bound by memory: a row is read once into registers, its sum of squares (and
+// for 8-bit output its largest magnitude) taken across the team of threads
+// that hold it, and every output written from the registers.  A team is a
+// wave up to 2,048 columns (four rows a workgroup, no barrier), a workgroup
+// of 256 or 1,024 threads beyond.
+
+#include "ffn_kernels.h"
+
+namespace bvml_ffn {
+
+namespace {
+
+constexpr int kVec = 8;  // columns a thread takes at a time
+constexpr float kE4M3Max = 448.0f;
+constexpr float kTiny = 1.17549435e-38f;  // 2^-126
+
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// Across the team: every thread gets the sum (the largest).  `turn` picks the
+// LDS slot, so that two reductions need one barrier each.
+template <int kTeam, typename T, typename Op>
+__device__ __forceinline__ T reduce(T v, Op op, T* slots) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = op(v, (T)__shfl_xor(v, d));
+    if constexpr (kTeam > 64) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) slots[w] = v;
+        __syncthreads();
+        v = slots[0];
+#pragma unroll
+        for (int j = 1; j < kTeam / 64; ++j) v = op(v, slots[j]);
+    }
+    return v;
+}
+
+template <int kTeam, int kV>
+__global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_kernel(NormCall c) {
+    __shared__ float sum_slots[kTeam / 64];
+    __shared__ uint32_t max_slots[kTeam / 64];
+    const int t = threadIdx.x % kTeam;
+    const long long row =
+        kTeam == 64 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long long)blockIdx.x;
+    if (row >= c.rows) return;  // whole teams
+    float v[kV][kVec];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+        const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+        if (left > 0) {
+            load_row<kVec>(c.x, c.x_type, row * c.ldx + col, left, v[k]);
+            if (c.residual) {
+                float r[kVec];
+                load_row<kVec>(c.residual, c.x_type, row * c.ldr + col, left, r);
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) v[k][i] += r[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) sum += v[k][i] * v[k][i];
+        }
+    }
+    sum = reduce<kTeam>(sum, [](float a, float b) { return a + b; }, sum_slots);
+    const float rstd = 1.0f / __builtin_sqrtf(sum / (float)c.cols + c.eps);
+    if (c.rstd && t == 0) c.rstd[row] = rstd;
+    // the largest |y|, compared as bits: a NaN is above every number
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+        const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+        if (left > 0) {
+            if (c.stream_out) store_row<kVec>(c.stream_out, c.x_type, row * c.lds + col, left, v[k]);
+            float w[kVec];
+            if (c.weight) {
+                load_row<kVec>(c.weight, c.w_type, col, left, w);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) w[i] = 1.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                v[k][i] = v[k][i] * rstd * w[i];
+                if (i < left)
+                    most = umax(most, __builtin_bit_cast(uint32_t, v[k][i]) & 0x7fffffffu);
+            }
+            if (c.y_type != kE4M3)
+                store_row<kVec>(c.y, c.y_type, row * c.ldy + col, left, v[k]);
+        }
+    }
+    if (c.y_type != kE4M3) return;
+    most = reduce<kTeam>(most, umax, max_slots);
+    const float top = __builtin_bit_cast(float, most) / kE4M3Max;
+    const float scale = top < kTiny ? kTiny : top;  // (a NaN stays)
+    if (t == 0) c.scale[row] = scale;
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+        const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+        if (left <= 0) continue;
+        int packed[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][4 * h] * inverse,
+                                                    v[k][4 * h + 1] * inverse, 0, false);
+            packed[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[k][4 * h + 2] * inverse,
+                                                        v[k][4 * h + 3] * inverse, p, true);
+        }
+        uint8_t* to = static_cast<uint8_t*>(c.y) + row * c.ldy + col;
+        if (left >= kVec) {
+            __builtin_memcpy(to, packed, 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+                if (i < left) to[i] = (uint8_t)((uint32_t)packed[i / 4] >> (8 * (i % 4)));
+        }
+    }
+}
+
+// A team walks rows `teams` apart and keeps its columns' part of the weight's
+// gradient in registers; a workgroup leaves one partial row.
+template <int kTeam, int kV>
+__global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_grad_kernel(NormGradCall c) {
+    constexpr int kTeams = kTeam == 64 ? 4 : 1;
+    __shared__ float slots[2][kTeam / 64];
+    __shared__ float sums[kTeam == 64 ? 3 : 1][kTeam == 64 ? kV * 64 * kVec : 1];
+    const int t = threadIdx.x % kTeam, team = kTeam == 64 ? threadIdx.x >> 6 : 0;
+    float dw[kV][kVec];
+#pragma unroll
+    for (int k = 0; k < kV; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) dw[k][i] = 0.0f;
+    int turn = 0;
+    for (long long row = (long long)blockIdx.x * kTeams + team; row < c.rows;
+         row += (long long)gridDim.x * kTeams) {
+        float n[kV][kVec], a[kV][kVec];
+        const float rstd = c.rstd[row];
+        float dot = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+            if (left > 0) {
+                float w[kVec];
+                load_row<kVec>(c.dy, c.dy_type, row * c.lddy + col, left, a[k]);
+                load_row<kVec>(c.stream_in, c.x_type, row * c.lds + col, left, n[k]);
+                if (c.weight) {
+                    load_row<kVec>(c.weight, c.w_type, col, left, w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) w[i] = 1.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    n[k][i] *= rstd;
+                    dw[k][i] += a[k][i] * n[k][i];
+                    a[k][i] *= w[i];
+                    dot += a[k][i] * n[k][i];
+                }
+            }
+        }
+        dot = reduce<kTeam>(dot, [](float x, float y) { return x + y; }, slots[turn]);
+        turn ^= 1;
+        const float mean = dot / (float)c.cols;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+            if (left > 0) {
+                float d[kVec];
+                if (c.dstream) {
+                    load_row<kVec>(c.dstream, c.x_type, row * c.ldds + col, left, d);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) d[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) d[i] += rstd * (a[k][i] - n[k][i] * mean);
+                store_row<kVec>(c.dx, c.x_type, row * c.lddx + col, left, d);
+            }
+        }
+    }
+    if (!c.dweight) return;
+    if constexpr (kTeam == 64) {
+        if (team != 0)
+#pragma unroll
+            for (int k = 0; k < kV; ++k)
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) sums[team - 1][(k * 64 + t) * kVec + i] = dw[k][i];
+        __syncthreads();
+        if (team != 0) return;
+#pragma unroll
+        for (int k = 0; k < kV; ++k)
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) dw[k][i] += sums[j][(k * 64 + t) * kVec + i];
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) {
+        const int col = (k * kTeam + t) * kVec, left = c.cols - col;
+        if (left > 0)
+            store_row<kVec>(c.workspace, kF32, (long long)blockIdx.x * c.cols + col, left, dw[k]);
+    }
+}
+
+int grad_blocks(int rows, int cols) {
+    const int teams = cols <= 2048 ? (rows + 3) / 4 : rows;
+    const int most = cols <= 2048 ? 1024 : 512;
+    return teams < most ? teams : most;
+}
+
+}  // namespace
+
+#define BVML_FFN_TEAMS(GO)                      \
+    if (cols <= 512) {                          \
+        GO(64, 1)                               \
+    } else if (cols <= 1024) {                  \
+        GO(64, 2)                               \
+    } else if (cols <= 1536) {                  \
+        GO(64, 3)                               \
+    } else if (cols <= 2048) {                  \
+        GO(64, 4)                               \
+    } else if (cols <= 4096) {                  \
+        GO(256, 2)                              \
+    } else if (cols <= 8192) {                  \
+        GO(256, 4)                              \
+    } else if (cols <= 16384) {                 \
+        GO(1024, 2)                             \
+    } else {                                    \
+        GO(1024, 4)                             \
+    }
+
+hipError_t launch_norm(const NormCall& c, hipStream_t s) {
+    const int cols = c.cols;
+#define BVML_FFN_GO(T, V)                                                                   \
+    hipLaunchKernelGGL((norm_kernel<T, V>), dim3((unsigned)(T == 64 ? (c.rows + 3) / 4 : c.rows)), \
+                       dim3(T == 64 ? 256 : T), 0, s, c);
+    BVML_FFN_TEAMS(BVML_FFN_GO)
+#undef BVML_FFN_GO
+    return hipGetLastError();
+}
+
+long long norm_grad_workspace(int rows, int cols) {
+    return (long long)grad_blocks(rows, cols) * cols * 4;
+}
+
+hipError_t launch_norm_grad(const NormGradCall& c, hipStream_t s) {
+    const int cols = c.cols, blocks = grad_blocks(c.rows, cols);
+    if (blocks > 0) {
+#define BVML_FFN_GO(T, V)                                                              \
+    hipLaunchKernelGGL((norm_grad_kernel<T, V>), dim3((unsigned)blocks),               \
+                       dim3(T == 64 ? 256 : T), 0, s, c);
+        BVML_FFN_TEAMS(BVML_FFN_GO)
+#undef BVML_FFN_GO
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return c.dweight ? launch_column_sum(c.workspace, blocks, cols, c.dweight, c.w_type, s)
+                     : hipSuccess;
+}
+
+}  // namespace bvml_ffn

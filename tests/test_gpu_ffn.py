@@ -1,0 +1,410 @@
+"""The feed-forward operators (brovisionml_amd/ffn.py, include/bvml_ffn.h) on
+the GPU against their definitions in double precision, within the bounds that
+tests/ffn_oracle.py derives: every kernel the launch plan can name, odd sizes,
+strided and misaligned rows, values that must not be read, gradients against
+the formulas and against differences, streams and graphs."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from brovisionml_amd import _lib, ffn
+from tests import ffn_oracle as orc
+
+pytestmark = pytest.mark.gpu
+BF, HF, FP, E4 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+CODE = {HF: _lib.F16, BF: _lib.BF16, E4: _lib.E4M3}
+
+
+def say(msg: str) -> None:
+    print("[gpu] " + msg, flush=True)
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return lambda *shape, std=1.0: torch.randn(shape, generator=g, device="cuda") * std
+
+
+def within(name, got, want, bound):
+    assert got.shape == want.shape, name
+    off = (got.double() - want).abs()
+    bad = ~(off <= bound)  # a NaN is outside
+    assert not bad.any(), (f"{name}: {int(bad.sum())} of {bad.numel()} outside, worst "
+                           f"{float((off / bound).nan_to_num(9e9).max()):.3g} of the bound")
+
+
+def inside(shape, dtype, pad=0, shift=0, fill=float("nan")):
+    """A tensor with `pad` more elements in every row, `shift` past its
+    allocation's start, all of them `fill`: (view, the allocation)."""
+    rows, cols = shape
+    big = torch.full((rows * (cols + pad) + shift + 64,), fill, device="cuda").to(dtype)
+    return torch.as_strided(big, shape, (cols + pad, 1), shift), big
+
+
+def put(t, pad=0, shift=0):
+    if not pad and not shift:
+        return t
+    v, _ = inside(t.shape, t.dtype, pad, shift)
+    v.copy_(t)
+    return v
+
+
+def quantised(v):
+    s = (v.abs().amax(-1) / 448).clamp(min=2.0 ** -126)
+    return (v / s[:, None]).to(E4), s
+
+
+# ---------------------------------------------------------------------------
+# linear and gated, forward
+# ---------------------------------------------------------------------------
+# M, N, K: the few-rows kernel with one, two and four blocks of rows; each
+# tile; split sums; sizes around a tile's and a step's edges
+FORWARD = [(1, 1, 1), (1, 1280, 5120), (3, 40, 72), (16, 16, 64), (17, 24, 200), (33, 50, 130),
+           (64, 1000, 1024), (65, 64, 64), (100, 136, 96), (129, 130, 1032), (252, 1000, 1024),
+           (300, 257, 264), (1000, 1111, 136), (1281, 2056, 520), (2100, 5128, 72),
+           (130, 5, 2048), (77, 513, 1), (200, 31, 33)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", FORWARD)
+def test_linear(cuda, M, N, K, dtype):
+    say(f"linear {M}x{K}x{N} {dtype}")
+    rnd = gen(M * 7 + N + K)
+    name = orc.ACTS[(M + N + K) % 5]
+    x, w = rnd(M, K).to(dtype), rnd(N, K, std=K ** -0.5).to(dtype)
+    b, r = rnd(N, std=0.3).to(dtype), rnd(M, N).to(dtype)
+    got = ffn.linear(x, w, b, name, r, save=True)
+    within("y", got.y, *orc.linear(x, w, b, name, r, dtype))
+    z, ez = orc.pre(x, w, b)
+    within("z", got.z, z, ez + orc.stored(z.abs() + ez, dtype))
+    within("plain", ffn.linear(x, w).y, *orc.linear(x, w, None, "none", None, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", FORWARD)
+def test_gated(cuda, M, N, K, dtype):
+    say(f"gated {M}x{K}x{N} {dtype}")
+    rnd = gen(M * 5 + N + K)
+    name = orc.ACTS[(M + N + K) % 5]
+    x, w = rnd(M, K).to(dtype), rnd(2 * N, K, std=K ** -0.5).to(dtype)
+    b = rnd(2 * N, std=0.3)
+    got = ffn.gated(x, w, b, name, save=True)
+    within("h", got.y, *orc.gated(x, w, b, name, dtype))
+    z, ez = orc.pre(x, w, b)
+    within("z", got.z, z, ez + orc.stored(z.abs() + ez, dtype))
+
+
+@pytest.mark.parametrize("name", orc.ACTS)
+def test_activations_over_their_range(cuda, name):
+    """Arguments from the far tails to zero, through a product with one term;
+    float32 output, so that only the activation's own error is there."""
+    say(f"activation {name}")
+    x = torch.cat([torch.linspace(-30, 30, 4801, device="cuda"),
+                   torch.tensor([0.0, -0.0, 1e-30, 300.0, -300.0], device="cuda")]).to(BF)[:, None]
+    one = torch.ones(1, 1, device="cuda", dtype=BF)
+    got = ffn.linear(x, one, act=name, dtype=FP).y
+    within(name, got, *orc.linear(x, one, None, name, None, FP))
+
+
+@pytest.mark.parametrize("out", [BF, HF, FP], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 64), (20, 33, 272), (64, 640, 1280), (70, 200, 144),
+                                   (300, 700, 400), (1400, 2000, 528), (9, 17, 5), (130, 70, 131),
+                                   (2100, 5128, 80)])
+def test_e4m3(cuda, M, N, K, out):
+    say(f"e4m3 {M}x{K}x{N} to {out}")
+    rnd = gen(M + N + K)
+    (x, xs), (w, ws) = quantised(rnd(M, K)), quantised(rnd(2 * N, K, std=K ** -0.5))
+    b, r = rnd(2 * N, std=0.2).to(out), rnd(M, N).to(out)
+    got = ffn.gated(x, w, b, "silu", x_scale=xs, w_scale=ws, dtype=out).y
+    within("gated", got, *orc.gated(x, w, b, "silu", out, xs, ws))
+    w, ws, b = w[:N], ws[:N], b[:N]
+    got = ffn.linear(x, w, b, "gelu", r, x_scale=xs, w_scale=ws, dtype=out).y
+    within("linear", got, *orc.linear(x, w, b, "gelu", r, out, xs, ws))
+
+
+# extra elements a row, elements before the first: rows of 16-byte steps, of
+# 4-byte steps, and at odd addresses; what lies between the rows is NaN
+@pytest.mark.parametrize("pad,shift", [(8, 8), (2, 2), (3, 1)])
+@pytest.mark.parametrize("M,N,K", [(5, 48, 64), (40, 30, 100), (150, 90, 136), (300, 260, 321)])
+def test_strided_rows_and_what_lies_between(cuda, M, N, K, pad, shift):
+    say(f"strided {M}x{K}x{N} pad {pad} shift {shift}")
+    rnd = gen(pad + M)
+    x, w = put(rnd(M, K).to(BF), pad, shift), put(rnd(N, K, std=K ** -0.5).to(BF), pad, shift)
+    r = put(rnd(M, N).to(BF), pad, shift)
+    out, big = inside((M, N), BF, pad, shift, fill=7.0)
+    before = big.clone()
+    got = ffn.linear(x, w, None, "silu", r, out=out).y
+    assert got is out
+    within("y", out, *orc.linear(x, w, None, "silu", r, BF))
+    out.copy_(torch.as_strided(before, out.shape, out.stride(), out.storage_offset()))
+    assert torch.equal(big, before), "written outside the output"
+    w2 = put(torch.cat([w, w]), pad, shift)
+    hout, big = inside((M, N), BF, pad, shift, fill=7.0)
+    before = big.clone()
+    ffn.gated(x, w2, None, "gelu", out=hout)
+    within("h", hout, *orc.gated(x, w2, None, "gelu", BF))
+    hout.copy_(torch.as_strided(before, hout.shape, hout.stride(), hout.storage_offset()))
+    assert torch.equal(big, before), "written outside the output"
+    # gradients of the same views
+    dy = put(rnd(M, N).to(BF), pad, shift)
+    for v, name in zip(zip(ffn.linear_backward(dy, x, w), orc.grads(dy, x, w, None, "none", False,
+                                                                    BF)), ("dx", "dw", "db")):
+        within(name, v[0], *v[1])
+    z = put(rnd(M, 2 * N).to(BF), pad, shift)
+    for v, name in zip(zip(ffn.gated_backward(dy, x, w2, z, "silu"),
+                           orc.grads(dy, x, w2, z, "silu", True, BF)), ("dx", "dw", "db")):
+        within("gated " + name, v[0], *v[1])
+
+
+def test_infinities_and_nans_stay_in_their_rows(cuda):
+    say("non-finite rows")
+    for M, K, N in ((6, 130, 50), (200, 136, 90)):
+        rnd = gen(M)
+        x, w = rnd(M, K).to(BF), rnd(N, K).to(BF)
+        x[1, 3], x[4, K - 1] = float("nan"), float("inf")
+        y = ffn.linear(x, w, act="none").y
+        want = x.float() @ w.float().t()
+        assert y[1].isnan().all()
+        assert torch.equal(y[4].isinf() | y[4].isnan(), want[4].isinf() | want[4].isnan())
+        keep = [i for i in range(M) if i not in (1, 4)]
+        assert y[keep].isfinite().all()
+
+
+def test_leading_dimensions_empty_batches_and_in_place_residual(cuda):
+    say("shapes")
+    rnd = gen(3)
+    x, w, r = rnd(3, 5, 64).to(BF), rnd(40, 64).to(BF), rnd(3, 5, 40).to(BF)
+    want, bound = orc.linear(x.reshape(15, 64), w, None, "none", r.reshape(15, 40), BF)
+    y = ffn.linear(x, w, residual=r, out=r).y
+    assert y.shape == (3, 5, 40) and y is r
+    within("y", y.reshape(15, 40), want, bound)
+    empty = x[:0]
+    assert ffn.linear(empty, w).y.shape == (0, 5, 40)
+    assert ffn.gated(empty, w).y.shape == (0, 5, 20)
+    n = ffn.add_rms_norm(empty, empty, save=True)
+    assert n.y.shape == (0, 5, 64) and n.rstd.shape == (0, 5)
+    dx, dw, db = ffn.linear_backward(r[:0], empty, w)
+    assert dx.shape == (0, 5, 64) and not dw.any() and not db.any()
+    dx, dw, db = ffn.gated_backward(r[:0, :, :20], empty, w, r[:0])
+    assert dx.shape == (0, 5, 64) and not dw.any() and not db.any()
+    weight = rnd(64).to(BF)
+    ds, dwt = ffn.add_rms_norm_backward(empty, empty, weight, torch.empty(0, 5, device="cuda"))
+    assert ds.shape == (0, 5, 64) and not dwt.any()
+    one = ffn.linear(x[0, 0], w).y  # a vector is one row
+    within("vector", one[None], *orc.linear(x[0, :1], w, None, "none", None, BF))
+
+
+# ---------------------------------------------------------------------------
+# gradients
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 40, 64), (7, 33, 50), (64, 64, 64),
+                                   (100, 130, 72), (333, 200, 1000), (1205, 341, 128),
+                                   (1000, 1283, 1100), (2300, 1290, 2304), (513, 2056, 4104),
+                                   (5000, 24, 40), (2700, 40, 4104)])
+def test_gradients(cuda, M, N, K, dtype):
+    say(f"gradients {M}x{K}x{N} {dtype}")
+    rnd = gen(M + 3 * N + K)
+    name = orc.ACTS[(M + N + K) % 5]
+    x, w = rnd(M, K).to(dtype), rnd(2 * N, K, std=K ** -0.5).to(dtype)
+    z, dy = rnd(M, 2 * N).to(dtype), rnd(M, N, std=0.3).to(dtype)
+    for which, got, want in zip(("dx", "dw", "db"), ffn.gated_backward(dy, x, w, z, name),
+                                orc.grads(dy, x, w, z, name, True, dtype)):
+        within("gated " + which, got, *want)
+    w, z = w[:N].contiguous(), z[:, :N].contiguous()
+    got = ffn.linear_backward(dy, x, w, z, name)
+    for which, g, want in zip(("dx", "dw", "db"), got, orc.grads(dy, x, w, z, name, False, dtype)):
+        within("linear " + which, g, *want)
+    f32 = rnd(M, N, std=0.3)
+    for which, g, want in zip(("dx", "dw", "db"), ffn.linear_backward(f32, x, w),
+                              orc.grads(f32, x, w, None, "none", False, dtype)):
+        within("float32 dy " + which, g, *want)
+    # each by itself is the same
+    only = ffn.linear_backward(dy, x, w, z, name, need_w=False, need_bias=False)
+    assert torch.equal(only[0], got[0]) and only[1] is None and only[2] is None
+    only = ffn.linear_backward(dy, x, w, z, name, need_x=False, need_bias=False)
+    assert torch.equal(only[1], got[1]) and only[0] is None
+
+
+@pytest.mark.parametrize("name", orc.ACTS)
+def test_gradients_against_differences(cuda, name):
+    """The whole block's gradients against central differences of its formula
+    in double precision along random directions."""
+    say(f"differences {name}")
+    rnd = gen(11)
+    M, K, N, h = 96, 72, 56, 1e-5
+    p = {"x": rnd(M, K), "r": rnd(M, K), "g": 1 + rnd(K, std=0.2), "wi": rnd(2 * N, K, std=0.12),
+         "wo": rnd(K, N, std=0.13), "bi": rnd(2 * N, std=0.3), "bo": rnd(K, std=0.3)}
+    p = {k: v.to(HF) for k, v in p.items()}
+    c = rnd(M, K, std=0.1).to(HF)
+    block = ffn.FeedForward(p["g"], p["wi"], p["wo"], p["bi"], p["bo"], act=name, eps=1e-5)
+    out, saved = block.forward(p["x"], p["r"], save=True)
+    got = block.backward(c, saved)
+
+    def loss(q):
+        s = q["x"] + q["r"]
+        y = s * torch.rsqrt((s * s).mean(-1, keepdim=True) + 1e-5) * q["g"]
+        g, u = (y @ q["wi"].t() + q["bi"]).chunk(2, -1)
+        o = s + (orc.act(name, g) * u) @ q["wo"].t() + q["bo"]
+        return (o * c.double()).sum()
+
+    d = {k: v.double() for k, v in p.items()}
+    assert (out.double() - (d["x"] + d["r"])).abs().max() > 0.1
+    for key, grad in (("x", "x"), ("r", "x"), ("g", "norm_weight"), ("wi", "w_in"),
+                      ("wo", "w_out"), ("bi", "b_in"), ("bo", "b_out")):
+        v = torch.sign(got[grad].double())  # along it, nothing cancels
+        along = float((loss({**d, key: d[key] + h * v}) - loss({**d, key: d[key] - h * v}))
+                      / (2 * h))
+        mine = float((got[grad].double() * v).sum())
+        # every 16-bit rounding on the way (s, y, z, h, dz, the gradient) is at most
+        # 2^-11 of its value; eight of them on either side of the products
+        assert abs(mine - along) <= 16 * 2.0 ** -11 * abs(along), (key, mine, along)
+
+
+# ---------------------------------------------------------------------------
+# the norm
+# ---------------------------------------------------------------------------
+NORM = [(1, 1), (1, 1280), (3, 7), (5, 64), (130, 513), (9, 1024), (6, 1025), (77, 1536),
+        (10, 1537), (5, 2048), (4, 2049), (3, 4097), (7, 8192), (2, 8195), (2, 20001), (1, 32768),
+        (4805, 128)]
+
+
+@pytest.mark.parametrize("xt,yt", [(BF, BF), (HF, HF), (FP, FP), (FP, BF), (FP, HF)])
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_norm(cuda, rows, cols, xt, yt):
+    say(f"norm {rows}x{cols} {xt} to {yt}")
+    rnd = gen(rows + cols)
+    x, r = rnd(rows, cols).to(xt), rnd(rows, cols, std=2.0).to(xt)
+    w = (1 + rnd(cols, std=0.3)).to(xt)
+    got = ffn.add_rms_norm(x, r, w, 1e-6, dtype=yt, save=True)
+    y, ey, s, es, rstd = orc.norm(x, r, w, 1e-6, xt)
+    within("y", got.y, y, ey + orc.stored(y.abs() + ey, yt))
+    within("stream", got.stream, s, es)
+    within("rstd", got.rstd, rstd, (cols + 16) * orc.F * rstd)
+    got = ffn.add_rms_norm(x, dtype=yt)
+    assert got.stream is x and got.rstd is None and got.scale is None
+    y, ey, _, _, _ = orc.norm(x, None, None, 1e-6, xt)
+    within("alone", got.y, y, ey + orc.stored(y.abs() + ey, yt))
+
+
+@pytest.mark.parametrize("xt", [BF, HF, FP], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_norm_to_e4m3(cuda, rows, cols, xt):
+    say(f"norm {rows}x{cols} {xt} to e4m3")
+    rnd = gen(rows + 2 * cols)
+    x, r, w = rnd(rows, cols).to(xt), rnd(rows, cols).to(xt), 1 + rnd(cols, std=0.3)
+    got = ffn.add_rms_norm(x, r, w, 1e-6, dtype=E4)
+    y, ey, s, es, _ = orc.norm(x, r, w, 1e-6, xt)
+    within("stream", got.stream, s, es)
+    top = y.abs().amax(-1) / 448
+    within("scale", got.scale, top, (cols + 24) * orc.F * top)
+    k = got.scale.double()[:, None]
+    # half a step of 3 mantissa bits, or of the subnormals' 2^-9
+    bound = ey + (y.abs() + ey) * 2.0 ** -4 + k * 2.0 ** -10 + 4 * orc.F * y.abs()
+    within("values", got.y.double() * k, y, bound)
+
+
+def test_norm_rows_of_zeros_and_nonfinite_rows(cuda):
+    say("norm edge rows")
+    x = torch.randn(4, 200, device="cuda")
+    x[0] = 0
+    x[1, 5], x[2, 7] = float("nan"), float("inf")
+    n = ffn.add_rms_norm(x, eps=1e-6)
+    assert not n.y[0].any() and n.y[1].isnan().all()
+    assert n.y[2, 7].isnan() and not n.y[2, :7].any() and n.y[3].isfinite().all()
+    q = ffn.add_rms_norm(x, eps=1e-6, dtype=E4)
+    v = q.y.float() * q.scale[:, None]
+    assert not v[0].any() and float(q.scale[0]) == 2.0 ** -126
+    assert v[1].isnan().all() and v[2].isnan().any() and v[3].isfinite().all()
+
+
+@pytest.mark.parametrize("xt,dt,wt", [(BF, BF, BF), (HF, HF, FP), (FP, BF, FP), (FP, FP, FP)])
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_norm_gradients(cuda, rows, cols, xt, dt, wt):
+    say(f"norm gradients {rows}x{cols} {xt} {dt} {wt}")
+    rnd = gen(rows + 5 * cols)
+    s, dy, dst = rnd(rows, cols, std=2.0).to(xt), rnd(rows, cols).to(dt), rnd(rows, cols).to(xt)
+    w = (1 + rnd(cols, std=0.3)).to(wt)
+    rstd = torch.rsqrt((s.float() ** 2).mean(-1) + 1e-6)
+    for d in (dst, None):
+        got = ffn.add_rms_norm_backward(dy, s, w, rstd, d)
+        want = orc.norm_grads(dy, s, w, rstd, d, xt, wt)
+        within("ds", got[0], *want[0])
+        within("dw", got[1], *want[1])
+    alone = ffn.add_rms_norm_backward(dy, s, None, rstd)
+    assert alone[1] is None
+    within("ds, no weight", alone[0], *orc.norm_grads(dy, s, None, rstd, None, xt, wt)[0])
+
+
+@pytest.mark.parametrize("pad,shift", [(8, 8), (2, 2), (3, 1)])
+@pytest.mark.parametrize("rows,cols", [(5, 64), (9, 77), (3, 2050)])
+def test_norm_strided(cuda, rows, cols, pad, shift):
+    say(f"norm strided {rows}x{cols} pad {pad} shift {shift}")
+    rnd = gen(cols)
+    x, r = put(rnd(rows, cols).to(BF), pad, shift), put(rnd(rows, cols).to(BF), pad, shift)
+    got = ffn.add_rms_norm(x, r, None, 1e-6, save=True)
+    y, ey, s, es, _ = orc.norm(x, r, None, 1e-6, BF)
+    within("y", got.y, y, ey + orc.stored(y.abs() + ey, BF))
+    within("stream", got.stream, s, es)
+    ds, _ = ffn.add_rms_norm_backward(x, r, None, got.rstd, x)
+    within("ds", ds, *orc.norm_grads(x, r, None, got.rstd, x, BF, BF)[0])
+
+
+# ---------------------------------------------------------------------------
+# together, on streams, in graphs
+# ---------------------------------------------------------------------------
+def _block(rnd, K, N, dtype):
+    return ffn.FeedForward((1 + rnd(K, std=0.1)).to(dtype), rnd(2 * N, K, std=K ** -0.5).to(dtype),
+                           rnd(K, N, std=N ** -0.5).to(dtype), rnd(2 * N, std=0.1).to(dtype),
+                           rnd(K, std=0.1).to(dtype))
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_equal_inputs_give_equal_bits_on_any_stream_and_in_a_graph(cuda, M):
+    say(f"block of {M} rows")
+    rnd = gen(M)
+    K, N = 264, 700
+    block = _block(rnd, K, N, BF)
+    x, r, c = rnd(M, K).to(BF), rnd(M, K).to(BF), rnd(M, K).to(BF)
+
+    def step():
+        out, saved = block.forward(x, r, save=True)
+        return [out, *block.backward(c, saved).values()]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        x.copy_(rnd(M, K).to(BF))
+        eager = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, captured)), k
+
+
+def test_long_rows_apart(cuda):
+    """Rows so far apart that element offsets pass 32 bits."""
+    say("offsets past 32 bits")
+    rows, cols, far = 600, 72, 4 * 1024 * 1024 - 256
+    big = torch.zeros(rows * far, dtype=BF, device="cuda")
+    x = torch.as_strided(big, (rows, cols), (far, 1))
+    rnd = gen(1)
+    x.copy_(rnd(rows, cols).to(BF))
+    w = rnd(48, cols, std=0.1).to(BF)
+    within("y", ffn.linear(x, w).y, *orc.linear(x, w, None, "none", None, BF))
+    n = ffn.add_rms_norm(x, x, save=True)
+    y, ey, _, _, _ = orc.norm(x, x, None, 1e-6, BF)
+    within("norm", n.y, y, ey + orc.stored(y.abs() + ey, BF))
+    dy = rnd(rows, 48).to(BF)
+    for which, got, want in zip(("dx", "dw", "db"), ffn.linear_backward(dy, x, w),
+                                orc.grads(dy, x, w, None, "none", False, BF)):
+        within(which, got, *want)
