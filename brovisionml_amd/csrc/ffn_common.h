@@ -32,10 +32,18 @@ __device__ __forceinline__ uint16_t to16(float v, int type) {
                          : __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 
+// A ragged end's own copy of a pointer: without it the compiler shares single
+// values between the two branches below and takes the whole vector apart.
+template <typename T>
+__device__ __forceinline__ T* apart(T* p) {
+    asm("" : "+v"(p));
+    return p;
+}
+
 // V consecutive values at element `at` of a 16- or 32-bit array, the first n
-// of them inside it (the others read as 0).  Whole vectors are one load of
-// up to 16 bytes at any alignment (the hardware takes unaligned global
-// accesses); only a row's ragged end goes value by value.
+// of them inside it (the others read as 0).  Whole vectors are loads of up to
+// 16 bytes at any alignment (the hardware takes unaligned global accesses);
+// only a row's ragged end goes value by value.
 template <int V>
 __device__ __forceinline__ void load_row(const void* base, int type, long long at, int n,
                                          float (&v)[V]) {
@@ -44,6 +52,7 @@ __device__ __forceinline__ void load_row(const void* base, int type, long long a
         if (n >= V) {
             __builtin_memcpy(v, p, 4 * V);
         } else {
+            p = apart(p);
 #pragma unroll
             for (int i = 0; i < V; ++i) v[i] = i < n ? p[i] : 0.0f;
         }
@@ -54,6 +63,7 @@ __device__ __forceinline__ void load_row(const void* base, int type, long long a
     if (n >= V) {
         __builtin_memcpy(h, p, 2 * V);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < V; ++i) h[i] = i < n ? p[i] : (uint16_t)0;
     }
@@ -69,6 +79,7 @@ __device__ __forceinline__ void store_row(void* base, int type, long long at, in
         if (n >= V) {
             __builtin_memcpy(p, v, 4 * V);
         } else {
+            p = apart(p);
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (i < n) p[i] = v[i];
@@ -82,6 +93,7 @@ __device__ __forceinline__ void store_row(void* base, int type, long long at, in
     if (n >= V) {
         __builtin_memcpy(p, h, 2 * V);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (i < n) p[i] = h[i];
@@ -190,56 +202,88 @@ struct Epilogue {
     int bias_type, out_type, z_type, act;
 };
 
-// V neighbouring sums of row m from column n on.
+// What a column adds, kept by the lane that finishes it.
 template <int V>
-__device__ __forceinline__ void affine(const Epilogue& e, int m, int col, int c, float (&v)[V]) {
-    if (e.x_scale) {
-        const float s = e.x_scale[m];
-        float w[V];
-        load_row<V>(e.w_scale, kF32, col, c, w);
+struct Column {
+    float bias[V], scale[V];
+    // columns col .. col + V, the first c of them inside
+    __device__ __forceinline__ void load(const Epilogue& e, int col, int c) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= s * w[i];
+        for (int i = 0; i < V; ++i) {
+            bias[i] = 0.0f;
+            scale[i] = 1.0f;
+        }
+        if (c <= 0) return;
+        if (e.bias) load_row<V>(e.bias, e.bias_type, col, c, bias);
+        if (e.w_scale) load_row<V>(e.w_scale, kF32, col, c, scale);
     }
-    if (e.bias) {
-        float b[V];
-        load_row<V>(e.bias, e.bias_type, col, c, b);
+    __device__ __forceinline__ void apply(float row_scale, float (&v)[V]) const {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] += b[i];
+        for (int i = 0; i < V; ++i) v[i] = v[i] * (row_scale * scale[i]) + bias[i];
     }
-}
+};
 
+// V neighbouring sums of row m from column n on, c of them inside; r: the
+// residual's values there (if any).  T: the 16-bit type, known to the kernel
+// where its operands are of it.
 template <int V>
-__device__ __forceinline__ void finish(const Epilogue& e, int m, int n, float (&v)[V]) {
-    const int c = e.N - n;
-    if (m >= e.M || c <= 0) return;
-    affine<V>(e, m, n, c, v);
-    if (e.z) store_row<V>(e.z, e.z_type, (long long)m * e.ldz + n, c, v);
+__device__ __forceinline__ void finish(const Epilogue& e, const Column<V>& k, int type16, int m,
+                                       int n, int c, float (&v)[V], const float (&r)[V]) {
+    k.apply(e.x_scale ? e.x_scale[m] : 1.0f, v);
+    if (e.z) store_row<V>(e.z, type16, (long long)m * e.ldz + n, c, v);
     activate<V>(e.act, v);
     if (e.residual) {
-        float r[V];
-        load_row<V>(e.residual, e.out_type, (long long)m * e.ldr + n, c, r);
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += r[i];
     }
-    store_row<V>(e.y, e.out_type, (long long)m * e.ldy + n, c, v);
+    store_row<V>(e.y, e.out_type == kF32 ? kF32 : type16, (long long)m * e.ldy + n, c, v);
 }
 
-// act(gate) * up for V neighbouring columns.
+// act(gate) * up.
 template <int V>
-__device__ __forceinline__ void finish_gated(const Epilogue& e, int m, int n, float (&g)[V],
-                                             float (&u)[V]) {
-    const int c = e.N - n;
-    if (m >= e.M || c <= 0) return;
-    affine<V>(e, m, n, c, g);
-    affine<V>(e, m, e.N + n, c, u);
+__device__ __forceinline__ void finish_gated(const Epilogue& e, const Column<V>& kg,
+                                             const Column<V>& ku, int type16, int m, int n, int c,
+                                             float (&g)[V], float (&u)[V]) {
+    const float s = e.x_scale ? e.x_scale[m] : 1.0f;
+    kg.apply(s, g);
+    ku.apply(s, u);
     if (e.z) {
-        store_row<V>(e.z, e.z_type, (long long)m * e.ldz + n, c, g);
-        store_row<V>(e.z, e.z_type, (long long)m * e.ldz + e.N + n, c, u);
+        store_row<V>(e.z, type16, (long long)m * e.ldz + n, c, g);
+        store_row<V>(e.z, type16, (long long)m * e.ldz + e.N + n, c, u);
     }
     activate<V>(e.act, g);
 #pragma unroll
     for (int i = 0; i < V; ++i) g[i] *= u[i];
-    store_row<V>(e.y, e.out_type, (long long)m * e.ldy + n, c, g);
+    store_row<V>(e.y, e.out_type == kF32 ? kF32 : type16, (long long)m * e.ldy + n, c, g);
+}
+
+// One vector by itself, for the kernels that finish few.
+template <int V>
+__device__ __forceinline__ void finish_one(const Epilogue& e, int type16, int m, int n,
+                                           float (&v)[V]) {
+    const int c = e.N - n;
+    if (m >= e.M || c <= 0) return;
+    Column<V> k;
+    k.load(e, n, c);
+    float r[V];
+    if (e.residual)
+        load_row<V>(e.residual, e.out_type == kF32 ? kF32 : type16, (long long)m * e.ldr + n, c, r);
+    finish<V>(e, k, type16, m, n, c, v, r);
+}
+template <int V>
+__device__ __forceinline__ void finish_one_gated(const Epilogue& e, int type16, int m, int n,
+                                                 float (&g)[V], float (&u)[V]) {
+    const int c = e.N - n;
+    if (m >= e.M || c <= 0) return;
+    Column<V> kg, ku;
+    kg.load(e, n, c);
+    ku.load(e, e.N + n, c);
+    finish_gated<V>(e, kg, ku, type16, m, n, c, g, u);
+}
+
+// The 16-bit type of a call: its operands' or, from 8 bits, its output's.
+__device__ __forceinline__ int type16_of(int in_type, const Epilogue& e) {
+    return in_type == kE4M3 ? e.out_type : in_type;
 }
 
 }  // namespace bvml_ffn

@@ -92,9 +92,7 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
                     } else {
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
-                            acc[h][b] = multiply16<kIn>(__builtin_bit_cast(v8s, qv[u][h][c]),
-                                                        __builtin_bit_cast(v8s, pv[u][b][c]),
-                                                        acc[h][b]);
+                            acc[h][b] = multiply16<kIn>(qv[u][h][c], pv[u][b][c], acc[h][b]);
                     }
                 }
     }
@@ -115,14 +113,14 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
     }
     const int m = 16 * w + i16, n = n0 + 4 * g;
     if constexpr (kGated)
-        finish_gated<4>(a.e, m, n, v[0], v[1]);
+        finish_one_gated<4>(a.e, type16_of(kIn, a.e), m, n, v[0], v[1]);
     else
-        finish<4>(a.e, m, n, v[0]);
+        finish_one<4>(a.e, type16_of(kIn, a.e), m, n, v[0]);
 }
 
 // Sums a split product's parts, in their order, and finishes them.
 template <bool kGated>
-__global__ __launch_bounds__(256) void join_kernel(Epilogue e, int splits) {
+__global__ __launch_bounds__(256) void join_kernel(Epilogue e, int in_type, int splits) {
     const int per = (e.N + 3) / 4;
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long m = t / per;
@@ -145,9 +143,9 @@ __global__ __launch_bounds__(256) void join_kernel(Epilogue e, int splits) {
         }
     }
     if constexpr (kGated)
-        finish_gated<4>(e, (int)m, n, v, u);
+        finish_one_gated<4>(e, type16_of(in_type, e), (int)m, n, v, u);
     else
-        finish<4>(e, (int)m, n, v);
+        finish_one<4>(e, type16_of(in_type, e), (int)m, n, v);
 }
 
 int step_of(int in_type) { return in_type == kE4M3 ? 128 : 64; }
@@ -258,9 +256,9 @@ hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s) 
     const long long threads = (long long)c.M * ((a.e.N + 3) / 4);
     const dim3 grid((unsigned)ceil_div(threads, 256));
     if (c.gated)
-        hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, s, a.e, p.splits);
+        hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, s, a.e, c.in_type, p.splits);
     else
-        hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, s, a.e, p.splits);
+        hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, s, a.e, c.in_type, p.splits);
     return hipGetLastError();
 }
 

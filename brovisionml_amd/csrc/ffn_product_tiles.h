@@ -25,9 +25,9 @@ template <int kIn, bool PT, bool QT, bool G>
 hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) {
     if (!p.dma) return launch_one<kIn, 128, 128, 2, 2, PT, QT, G, false>(a, p.splits, s);
     switch (p.tile) {
-        case kTile256: return launch_one<kIn, 256, 256, 2, 4, PT, QT, G, true>(a, p.splits, s);
+        case kTile256: return launch_one<kIn, 256, 256, 2, 2, PT, QT, G, true>(a, p.splits, s);
         case kTile128: return launch_one<kIn, 128, 128, 2, 2, PT, QT, G, true>(a, p.splits, s);
-        default: return launch_one<kIn, 64, 64, 2, 2, PT, QT, G, true>(a, p.splits, s);
+        default: return launch_one<kIn, 64, 128, 2, 2, PT, QT, G, true>(a, p.splits, s);
     }
 }
 
