@@ -239,7 +239,7 @@ def load_ffn(path: str = LIB_FFN) -> ctypes.CDLL:
     for name in ("bvml_ffn_linear_backward", "bvml_ffn_gated_backward"):
         getattr(lib, name).argtypes = [vp, ll, vp, ll, vp, ll, vp, ll, i, i, i, i, i, i, vp, ll, vp,
                                        ll, vp, vp, ll, vp]
-    lib.bvml_ffn_plan.argtypes = [i, i, i, i, i, i, i, ip, ip, ip]
+    lib.bvml_ffn_plan.argtypes = [i, i, i, i, i, i, i, ip, ip, ip, ip]
     for name in ("bvml_ffn_add_rms_norm", "bvml_ffn_add_rms_norm_backward", "bvml_ffn_linear",
                  "bvml_ffn_gated", "bvml_ffn_linear_backward", "bvml_ffn_gated_backward",
                  "bvml_ffn_plan"):
@@ -266,15 +266,16 @@ def ffn_last_error() -> str:
 
 def ffn_plan(M: int, R: int, K: int, in_type: int, layout: int = 0, gated: bool = False,
              aligned: bool = True):
-    """(rows of a tile (0: the few-rows kernel), operands straight to LDS?,
-    parts of the sum) of a product of C (M, R) over K; raises on a rejected
-    argument."""
-    tile, dma, splits = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    """(rows of a tile (0: the few-rows kernel), four LDS slots?, tiles that one
+    workgroup sums, workgroups for each of the others) of a product of C
+    (M, R) over K; raises on a rejected argument."""
+    out = [ctypes.c_int() for _ in range(4)]
     st = load_ffn().bvml_ffn_plan(M, R, K, in_type, layout, int(gated), int(aligned),
-                                  ctypes.byref(tile), ctypes.byref(dma), ctypes.byref(splits))
+                                  *(ctypes.byref(v) for v in out))
     if st != OK:
         raise RuntimeError(f"ffn_plan: {ffn_last_error()} (status {st})")
-    return tile.value, bool(dma.value), splits.value
+    tile, deep, whole, splits = (v.value for v in out)
+    return tile, bool(deep), whole, splits
 
 
 def refine_last_error() -> str:

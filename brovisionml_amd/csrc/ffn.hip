@@ -161,7 +161,9 @@ struct GradSpace {
         sums = round256(slope_workspace(M, R));
         const long long a = product_workspace(M, K, R, type, kInputGrad, false);
         const long long b = product_workspace(R, K, M, type, kWeightGrad, false);
+        const long long c = gradients_workspace(M, R, K);
         parts = a > b ? a : b;
+        if (c > parts) parts = c;
     }
     long long all() const { return dz + sums + parts; }
 };
@@ -226,29 +228,29 @@ int backward(const std::string& op, bool gated, const void* dy, long long lddy, 
     c.in_type = type;
     c.gated = false;
     c.padded_p = own_dz;
+    auto plain = [&](void* y, long long ldy, int rows) {
+        return Epilogue{nullptr, nullptr, nullptr, nullptr, y, nullptr, nullptr, 0, ldy, 0, rows, K,
+                        type, type, type, BVML_FFN_NONE};
+    };
+    ProductCall input = c, weight = c;
+    input.q = w;
+    input.ldq = ldw;
+    input.M = M;
+    input.R = K;
+    input.K = R;
+    input.layout = kInputGrad;
+    input.e = plain(dx, lddx, M);
+    weight.q = x;
+    weight.ldq = ldx;
+    weight.M = R;
+    weight.R = K;
+    weight.K = M;
+    weight.layout = kWeightGrad;
+    weight.e = plain(dw, lddw, R);
     void* const parts = at + space.dz + space.sums;
-    if (dx && M > 0) {
-        c.q = w;
-        c.ldq = ldw;
-        c.M = M;
-        c.R = K;
-        c.K = R;
-        c.layout = kInputGrad;
-        c.e = Epilogue{nullptr, nullptr, nullptr, nullptr, dx, nullptr, nullptr, 0, lddx, 0, M, K,
-                       type, type, type, BVML_FFN_NONE};
-        BVML_FFN_TRY(launched(op, launch_product(c, parts, s)));
-    }
-    if (dw) {
-        c.q = x;
-        c.ldq = ldx;
-        c.M = R;
-        c.R = K;
-        c.K = M;
-        c.layout = kWeightGrad;
-        c.e = Epilogue{nullptr, nullptr, nullptr, nullptr, dw, nullptr, nullptr, 0, lddw, 0, R, K,
-                       type, type, type, BVML_FFN_NONE};
-        BVML_FFN_TRY(launched(op, launch_product(c, parts, s)));
-    }
+    if (dx && dw) return launched(op, launch_gradients(input, weight, parts, s));
+    if (dx && M > 0) return launched(op, launch_product(input, parts, s));
+    if (dw) return launched(op, launch_product(weight, parts, s));
     return BVML_FFN_OK;
 }
 
@@ -388,16 +390,23 @@ long long bvml_ffn_gated_backward_workspace(int M, int N, int K) {
 }
 
 int bvml_ffn_plan(int M, int R, int K, int in_type, int layout, int gated, int aligned, int* tile,
-                  int* dma, int* splits) {
+                  int* deep, int* whole, int* splits) {
     if (M < 1 || R < 1 || K < 1)
         return fail(BVML_FFN_ESHAPE, "plan: sizes must be >= 1");
-    if ((in_type != kE4M3 && !is16(in_type)) || layout < kForward || layout > kWeightGrad ||
+    if ((in_type != kE4M3 && !is16(in_type)) || layout < kForward || layout > kWeightGrad + 1 ||
         (layout != kForward && (gated || in_type == kE4M3)))
         return fail(BVML_FFN_ETYPE, "plan: no such product");
-    const ProductPlan p = plan_product(M, R, K, in_type, layout, gated != 0, aligned != 0);
-    if (tile)
-        *tile = p.tile == kTile256 ? 256 : p.tile == kTile128 ? 128 : p.tile == kTile64 ? 64 : 0;
-    if (dma) *dma = p.dma;
+    ProductPlan p;
+    if (layout <= kWeightGrad) {
+        p = plan_product(M, R, K, in_type, layout, gated != 0, aligned != 0);
+    } else {
+        const GradientsPlan g = plan_gradients(M, R, K);
+        p = {g.tile, true, g.input_splits > 1 ? g.input_whole : g.weight_whole,
+             g.input_splits > 1 ? g.input_splits : g.weight_splits};
+    }
+    if (tile) *tile = p.tile == kTileRows ? 0 : p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128;
+    if (deep) *deep = p.tile == kTile128Deep;
+    if (whole) *whole = p.whole;
     if (splits) *splits = p.splits;
     return BVML_FFN_OK;
 }

@@ -257,29 +257,32 @@ __device__ __forceinline__ void finish_gated(const Epilogue& e, const Column<V>&
     store_row<V>(e.y, e.out_type == kF32 ? kF32 : type16, (long long)m * e.ldy + n, c, g);
 }
 
-// One vector by itself, for the kernels that finish few.
-template <int V>
-__device__ __forceinline__ void finish_one(const Epilogue& e, int type16, int m, int n,
-                                           float (&v)[V]) {
-    const int c = e.N - n;
-    if (m >= e.M || c <= 0) return;
-    Column<V> k;
-    k.load(e, n, c);
+// One vector by itself, for the kernels that finish few: what it adds, asked
+// for before the sums are there, then the rest.
+template <int V, bool kGated>
+struct Single {
+    Column<V> k, ku;
     float r[V];
-    if (e.residual)
-        load_row<V>(e.residual, e.out_type == kF32 ? kF32 : type16, (long long)m * e.ldr + n, c, r);
-    finish<V>(e, k, type16, m, n, c, v, r);
-}
-template <int V>
-__device__ __forceinline__ void finish_one_gated(const Epilogue& e, int type16, int m, int n,
-                                                 float (&g)[V], float (&u)[V]) {
-    const int c = e.N - n;
-    if (m >= e.M || c <= 0) return;
-    Column<V> kg, ku;
-    kg.load(e, n, c);
-    ku.load(e, e.N + n, c);
-    finish_gated<V>(e, kg, ku, type16, m, n, c, g, u);
-}
+    __device__ __forceinline__ void load(const Epilogue& e, int type16, int m, int n) {
+        const int c = e.N - n;
+        if (m >= e.M || c <= 0) return;
+        k.load(e, n, c);
+        if constexpr (kGated) ku.load(e, e.N + n, c);
+        if (!kGated && e.residual)
+            load_row<V>(e.residual, e.out_type == kF32 ? kF32 : type16,
+                        (long long)m * e.ldr + n, c, r);
+    }
+    // v: the sums (gated: the gate's), u: the other half's
+    __device__ __forceinline__ void finish(const Epilogue& e, int type16, int m, int n,
+                                           float (&v)[V], float (&u)[V]) const {
+        const int c = e.N - n;
+        if (m >= e.M || c <= 0) return;
+        if constexpr (kGated)
+            finish_gated<V>(e, k, ku, type16, m, n, c, v, u);
+        else
+            bvml_ffn::finish<V>(e, k, type16, m, n, c, v, r);
+    }
+};
 
 // The 16-bit type of a call: its operands' or, from 8 bits, its output's.
 __device__ __forceinline__ int type16_of(int in_type, const Epilogue& e) {

@@ -23,12 +23,15 @@ struct ProductCall {
     Epilogue e;
 };
 
-enum Tile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTileRows = 3 };
+// 256 x 256; 128 x 128 with two LDS slots (two workgroups a CU) or four (one);
+// 64 x 128 with three (two a CU); the few-rows kernel.
+enum Tile { kTile256 = 0, kTile128 = 1, kTile128Deep = 2, kTile64 = 3, kTileRows = 4 };
 
 struct ProductPlan {
-    int tile;    // a Tile; kTileRows: the few-rows kernel
+    int tile;    // a Tile
     bool dma;    // copies go straight to LDS
-    int splits;  // the sum's parts, joined by a second launch
+    int whole;   // tiles that one workgroup sums
+    int splits;  // workgroups for each of the others, joined by a second launch
 };
 
 // The kernel for a product of these sizes (dma: dma_fits of its operands).
@@ -38,6 +41,19 @@ bool dma_fits(const ProductCall& c);
 long long product_workspace(int M, int R, int K, int in_type, int layout, bool gated);
 hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s);
 
+// Both gradients of one product from the same dz: x's (c.p = dz, c.q = W) and W's
+// (c.p = dz, c.q = x), in one launch where their operands go straight to LDS.
+struct GradientsPlan {
+    int tile;
+    bool weight_first;  // the weight's workgroups take longer
+    // tiles of each that one workgroup sums, workgroups for each of the others
+    int input_whole, input_splits, weight_whole, weight_splits;
+};
+GradientsPlan plan_gradients(int M, int R, int K);
+long long gradients_workspace(int M, int R, int K);
+hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight, void* workspace,
+                            hipStream_t s);
+
 // One translation unit an element type (ffn_product_*.hip).
 struct Product;
 hipError_t launch_tiles_f16(const Product& a, const ProductPlan& p, int layout, bool gated,
@@ -46,6 +62,10 @@ hipError_t launch_tiles_bf16(const Product& a, const ProductPlan& p, int layout,
                              hipStream_t s);
 hipError_t launch_tiles_e4m3(const Product& a, const ProductPlan& p, int layout, bool gated,
                              hipStream_t s);
+struct Gradients;
+hipError_t launch_gradients_f16(const Gradients& g, int tile, hipStream_t s);
+hipError_t launch_gradients_bf16(const Gradients& g, int tile, hipStream_t s);
+
 struct NormCall {
     const void* x;
     const void* residual;

@@ -48,8 +48,10 @@ struct Product {
     int M, K;               // C's rows; the sum's length
     int R;                  // Q's columns of C: N, or 2N for the gated form
     int tiles_m, tiles_n;
-    int steps;              // ceil(K / kStep): all of them
-    int per_split;          // steps a workgroup takes (blockIdx.y: which)
+    int steps;              // ceil(K / kStep)
+    // The first `whole` tiles have a workgroup each; each of the others has
+    // `splits`, for per_split steps each, which leave fp32 parts of the tile.
+    int whole, splits, per_split;
     Epilogue e;
 };
 
@@ -231,24 +233,27 @@ struct Copy {
     }
 };
 
-// The tile of workgroup `b` of n: consecutive tiles on one XCD (workgroups go
-// round the 8 of them), so that its L2 serves the operand rows they share,
-// and within that groups of kGroup row tiles by all column tiles.
-constexpr int kXcds = 8;
+// Tile t of a product: groups of kGroup row tiles by all column tiles, so that
+// neighbours share operand rows.
 constexpr int kGroup = 4;
-
-__device__ __forceinline__ void tile_of(int b, int tm, int tn, int& m, int& n) {
-    const int total = tm * tn, each = total / kXcds, more = total % kXcds;
-    const int x = b % kXcds, i = b / kXcds;
-    const int t = x * each + (x < more ? x : more) + i;
+__device__ __forceinline__ void tile_of(int t, int tm, int tn, int& m, int& n) {
     const int per = kGroup * tn, g = t / per, in = t % per;
     const int rows = tm - g * kGroup < kGroup ? tm - g * kGroup : kGroup;
     m = g * kGroup + in % rows;
     n = in / rows;
 }
+// Workgroup b of n as a place in the tiles' order: consecutive tiles on one
+// XCD (workgroups go round the 8 of them), whose L2 then serves them all.
+constexpr int kXcds = 8;
+__device__ __forceinline__ int place_of(int b, int n) {
+    const int each = n / kXcds, more = n % kXcds, x = b % kXcds;
+    return x * each + (x < more ? x : more) + b / kXcds;
+}
 
-template <int kIn, int BM, int BN, int WM, int WN, bool kPT, bool kQT, bool kGated, bool kDma>
-__global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product_kernel(Product a) {
+// One workgroup's tile: workgroup b of the product's, LDS of kLdsBytes.
+template <int kIn, int BM, int BN, int kSlots, bool kPT, bool kQT, bool kGated, bool kDma>
+__device__ __forceinline__ void product_tile(const Product& a, const int b, char* const lds) {
+    constexpr int WM = 2, WN = 2;
     constexpr int kWaves = WM * WN;
     constexpr int MT = BM / WM, NT = BN / WN, MB = MT / 32, NB = NT / 32;
     constexpr int kSize = kIn == kE4M3 ? 1 : 2;
@@ -257,16 +262,19 @@ __global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product
     static_assert(!kGated || NB % 2 == 0, "");
     static_assert(!(kGated && kQT) && !((kPT || kQT) && kIn == kE4M3), "");
 
-    __shared__ __align__(1024) char lds[2 * kSlot];
-
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = w / WN, wn = w % WN;
-    int tm, tn;
-    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    int tm, tn, step0 = 0, step1 = a.steps;
+    const bool part = b >= a.whole;
+    if (!part) {
+        tile_of(place_of(b, a.whole), a.tiles_m, a.tiles_n, tm, tn);
+    } else {
+        tile_of(a.whole + (b - a.whole) / a.splits, a.tiles_m, a.tiles_n, tm, tn);
+        step0 = (b - a.whole) % a.splits * a.per_split;
+        step1 = step0 + a.per_split < a.steps ? step0 + a.per_split : a.steps;
+    }
     const int m0 = tm * BM, n0 = tn * (kGated ? BN / 2 : BN);
-    const int step0 = blockIdx.y * a.per_split;
-    const int step1 = step0 + a.per_split < a.steps ? step0 + a.per_split : a.steps;
 
     // ---- copies
     using CopyP = Copy<kIn, BM, kWaves, kPT, false, kDma>;
@@ -384,35 +392,43 @@ __global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product
                 qq[j] = along(s + qrow(j), qat[0] ^ (kk * 64));
         }
     };
-    // this wave's copies landed and its reads done, then every wave's
+    // The next step's copies of this wave landed (those of the steps after it
+    // may be on their way) and its reads are done; then every wave's.
+    constexpr int kCopies = PP + QP, kFlying = (kSlots - 2) * kCopies;
+    static_assert(kFlying < 64, "what vmcnt can count");
     auto arrive = [&]() {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(kDma ? 0x0070 : 0xc07f);  // vmcnt(0) lgkmcnt(0), or lgkmcnt(0)
+        __builtin_amdgcn_s_waitcnt(kDma ? 0x0070 | (kFlying & 15) | (kFlying >> 4 << 14) : 0xc07f);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
     // The products of a half in kGroups groups; between them the next half's
     // reads, in the groups' first half, and copies.
     constexpr int kKs = kIn == kE4M3 ? 1 : 2, kGroups = MB * NB;
-    constexpr int kReads = MB + NB, kCopies = PP + QP;
+    constexpr int kReads = MB + NB;
+    static_assert(kDma || kSlots == 2, "one step in registers");
 
     if (step0 < step1) {
+        // (past the last step a copy is zeros: every step counts the same)
         start_all(step0, lds);
         commit(lds);
+#pragma unroll
+        for (int i = 1; i < kSlots - 1; ++i) start_all(step0 + i, lds + i * kSlot);
         arrive();
-        start_all(step0 + 1, lds + kSlot);
+        start_all(step0 + kSlots - 1, lds + (kSlots - 1) * kSlot);
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(lds, 0, r, p[0], q[0]);
         int cur = 0;
         for (int s = step0; s < step1; ++s) {
+            const int next = cur == (kSlots - 1) * kSlot ? 0 : cur + kSlot;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 if (kk == 1) {
-                    commit(lds + (cur ^ kSlot));
+                    commit(lds + next);
                     arrive();
-                    aim(s + 2);
+                    aim(s + kSlots);
                 }
-                const char* const from = lds + (kk == 0 ? cur : cur ^ kSlot);
+                const char* const from = lds + (kk == 0 ? cur : next);
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) {
 #pragma unroll
@@ -432,7 +448,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            cur ^= kSlot;
+            cur = next;
         }
         // no copy may be in flight when the workgroup's LDS is given away
         if constexpr (kDma) __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -440,59 +456,32 @@ __global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product
 
     // ---- epilogue, 32 rows of the wave's part at a time: the sums go through
     // LDS, so that a row of C is finished by neighbouring lanes, 8 columns
-    // each, in one rolled loop.  (Straight from the registers it is thousands
+    // each, in a rolled loop.  (Straight from the registers it is thousands
     // of instructions that run once, and fetching them costs more than the
     // products: a 256 x 256 tile took 100 us.)
     __builtin_amdgcn_s_barrier();  // every wave has read its last operands
     asm volatile("" ::: "memory");
     constexpr int kPitch = NT + 4;  // floats; rows 16 bytes apart in the banks
-    static_assert(32 * kPitch * 4 * kWaves <= (int)sizeof(lds), "");
+    static_assert(32 * kPitch * 4 * kWaves <= kSlots * kSlot, "");
     float* const sums = reinterpret_cast<float*>(lds) + w * 32 * kPitch;
     const Epilogue& e = a.e;
-    const bool part = gridDim.y > 1;
+    constexpr bool kPlain = kPT || kQT;  // a gradient: nothing but the store
     constexpr int kCols = kGated ? NT / 2 : NT, kLanes = kCols / 8;  // lanes of a row
-    constexpr int kRowsAtOnce = 64 / kLanes, kTimes = 32 / kRowsAtOnce;
+    // the lane takes every kGap-th row, kTimes rows at once
+    constexpr int kGap = 64 / kLanes, kTimes = 32 / kGap < 4 ? 32 / kGap : 4;
     const int type16 = kIn == kE4M3 ? e.out_type : kIn;
+    const int y_type = e.out_type == kF32 ? kF32 : type16;
     const int row0 = lane / kLanes, col = lane % kLanes * 8, n = n0 + wn * kCols + col;
     const int c = e.N - n;
+    // no ragged column and no row beyond the last in the tile
+    const bool whole = n0 + (kGated ? BN / 2 : BN) <= e.N && m0 + BM <= a.M;
     Column<8> kv, ku;
-    if (!part) {
+    if (!kPlain && !part) {
         kv.load(e, n, c);
         if constexpr (kGated) ku.load(e, e.N + n, c);
     }
-    // rows of the wave's part from 32 i on, their columns whole or ragged
-    auto rows = [&](int i, int m, float (&v)[8], const float (&r)[8], int inside) {
-        float u[8];
-        const float* const at = sums + (m - (m0 + wm * MT + 32 * i)) * kPitch + col;
-        __builtin_memcpy(v, __builtin_assume_aligned(at, 16), 32);
-        if constexpr (kGated) __builtin_memcpy(u, __builtin_assume_aligned(at + kCols, 16), 32);
-        if (part) {
-            const long long to = ((long long)blockIdx.y * a.M + m) * a.R + n;
-            store_row<8>(e.part, kF32, to, inside, v);
-            if constexpr (kGated) store_row<8>(e.part, kF32, to + e.N, inside, u);
-        } else if constexpr (kGated) {
-            finish_gated<8>(e, kv, ku, type16, m, n, inside, v, u);
-        } else {
-            finish<8>(e, kv, type16, m, n, inside, v, r);
-        }
-    };
-    const bool whole = n0 + (wn + 1) * kCols <= e.N;
 #pragma unroll 1
     for (int i = 0; i < MB; ++i) {
-        // the residual's rows first: they arrive while the sums change places
-        const int first = m0 + wm * MT + 32 * i + row0;
-        float r[kGated ? 1 : kTimes][8];
-        if constexpr (!kGated && !kQT) {
-            if (e.residual && whole && !part) {
-                const int type = e.out_type == kF32 ? kF32 : type16;
-#pragma unroll
-                for (int t = 0; t < kTimes; ++t) {
-                    const int m = first + t * kRowsAtOnce;
-                    load_row<8>(e.residual, type, (long long)(m < a.M ? m : a.M - 1) * e.ldr + n, 8,
-                                r[t]);
-                }
-            }
-        }
 #pragma unroll
         for (int x = 0; x < MB; ++x) {
             if (x != i) continue;
@@ -504,27 +493,136 @@ __global__ __launch_bounds__(64 * WM * WN, BM* BN >= 65536 ? 1 : 2) void product
                         (v4f){acc[x][j][y], acc[x][j][y + 1], acc[x][j][y + 2], acc[x][j][y + 3]};
         }
         asm volatile("" ::: "memory");
-        if (whole) {
+#pragma unroll 1
+        for (int from = row0; from < 32; from += kTimes * kGap) {
+            const int first = m0 + wm * MT + 32 * i + from;
+            // each step for all of the lane's rows before the next: one branch a step
+            auto store = [&](void* to, int type, long long ld, int at, const float (&x)[kTimes][8]) {
+                const int size = type == kF32 ? 4 : 2;
+                char* p = static_cast<char*>(to) + ((long long)first * ld + at) * size;
+                const long long step = kGap * ld * size;
+                if (whole) {
+#pragma unroll
+                    for (int t = 0; t < kTimes; ++t, p += step) store_row<8>(p, type, 0, 8, x[t]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < kTimes; ++t, p += step)
+                        if (first + t * kGap < a.M && c > 0) store_row<8>(p, type, 0, c, x[t]);
+                }
+            };
+            float r[kPlain || kGated ? 1 : kTimes][8];
+            if constexpr (!kPlain && !kGated) {
+                if (e.residual && !part) {
+#pragma unroll
+                    for (int t = 0; t < kTimes; ++t) {
+                        const int m = first + t * kGap;
+                        const long long at = (long long)(m < a.M ? m : a.M - 1) * e.ldr + n;
+                        if (whole)
+                            load_row<8>(e.residual, y_type, at, 8, r[t]);
+                        else
+                            load_row<8>(e.residual, y_type, at, c, r[t]);
+                    }
+                }
+            }
+            float v[kTimes][8], u[kGated ? kTimes : 1][8];
 #pragma unroll
             for (int t = 0; t < kTimes; ++t) {
-                const int m = first + t * kRowsAtOnce;
-                float v[8];
-                if (m < a.M) rows(i, m, v, r[kGated ? 0 : t], 8);
+                const float* const at = sums + (from + t * kGap) * kPitch + col;
+                __builtin_memcpy(v[t], __builtin_assume_aligned(at, 16), 32);
+                if constexpr (kGated)
+                    __builtin_memcpy(u[t], __builtin_assume_aligned(at + kCols, 16), 32);
             }
-        } else {
-#pragma unroll 1
-            for (int t = 0; t < kTimes; ++t) {
-                const int m = first + t * kRowsAtOnce;
-                float v[8], s[8];
-                if (m >= a.M || c <= 0) continue;
-                if (e.residual && !part)
-                    load_row<8>(e.residual, e.out_type == kF32 ? kF32 : type16,
-                                (long long)m * e.ldr + n, c, s);
-                rows(i, m, v, s, c);
+            if (part) {
+                // the workgroup's own BM x BN floats, whole also at the edges
+                float* to = e.part + (long long)(b - a.whole) * BM * BN +
+                            (wm * MT + 32 * i + from) * BN + wn * kCols + col;
+#pragma unroll
+                for (int t = 0; t < kTimes; ++t, to += kGap * BN) {
+                    store_row<8>(to, kF32, 0, 8, v[t]);
+                    if constexpr (kGated) store_row<8>(to, kF32, BN / 2, 8, u[t]);
+                }
+                continue;
             }
+            if constexpr (!kPlain) {
+#pragma unroll
+                for (int t = 0; t < kTimes; ++t) {
+                    const int m = first + t * kGap;
+                    const float s = e.x_scale ? e.x_scale[m < a.M ? m : a.M - 1] : 1.0f;
+                    kv.apply(s, v[t]);
+                    if constexpr (kGated) ku.apply(s, u[t]);
+                }
+                if (e.z) {
+                    store(e.z, type16, e.ldz, n, v);
+                    if constexpr (kGated) store(e.z, type16, e.ldz, e.N + n, u);
+                }
+                activate<8 * kTimes>(e.act, reinterpret_cast<float(&)[8 * kTimes]>(v));
+                if constexpr (kGated) {
+#pragma unroll
+                    for (int t = 0; t < kTimes; ++t)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) v[t][x] *= u[t][x];
+                } else if (e.residual) {
+#pragma unroll
+                    for (int t = 0; t < kTimes; ++t)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) v[t][x] += r[t][x];
+                }
+            }
+            if (y_type == kF32)
+                store(e.y, kF32, e.ldy, n, v);
+            else
+                store(e.y, type16, e.ldy, n, v);
         }
         asm volatile("" ::: "memory");
     }
+}
+
+template <int BM, int BN, int kSlots>
+constexpr int kLdsBytes = kSlots * (BM + BN) * 128;
+// (the 256 x 256 tile's sums take 256 registers a lane)
+template <int BM>
+constexpr int kWavesPerSimd = BM == 256 ? 1 : 2;
+
+template <int kIn, int BM, int BN, int kSlots, bool kPT, bool kQT, bool kGated, bool kDma>
+__global__ __launch_bounds__(256, kWavesPerSimd<BM>) void product_kernel(Product a) {
+    __shared__ __align__(1024) char lds[kLdsBytes<BM, BN, kSlots>];
+    product_tile<kIn, BM, BN, kSlots, kPT, kQT, kGated, kDma>(a, blockIdx.x, lds);
+}
+
+// Both gradients of a product in one launch, so that one's tiles fill the CUs
+// that the other's leave idle.  The product whose workgroups take longer goes
+// first, for a long one started last would keep the launch waiting; before it
+// the parts of the other's last tiles, where only those are split.
+struct Gradients {
+    Product input, weight;
+    bool weight_first;
+};
+
+__device__ __forceinline__ int rest_of(const Product& a) {
+    return (a.tiles_m * a.tiles_n - a.whole) * a.splits;
+}
+
+template <int kIn, int BM, int BN, int kSlots>
+__global__ __launch_bounds__(256, kWavesPerSimd<BM>) void gradients_kernel(Gradients g) {
+    __shared__ __align__(1024) char lds[kLdsBytes<BM, BN, kSlots>];
+    const Product& first = g.weight_first ? g.weight : g.input;
+    const Product& second = g.weight_first ? g.input : g.weight;
+    const int parts = second.whole > 0 ? rest_of(second) : 0;
+    const int longer = first.whole + rest_of(first);
+    int b = blockIdx.x;
+    bool weight = !g.weight_first;
+    if (b < parts) {
+        b += second.whole;
+    } else if (b < parts + longer) {
+        b -= parts;
+        weight = g.weight_first;
+    } else {
+        b -= parts + longer;
+    }
+    if (weight)
+        product_tile<kIn, BM, BN, kSlots, true, true, false, true>(g.weight, b, lds);
+    else
+        product_tile<kIn, BM, BN, kSlots, false, true, false, true>(g.input, b, lds);
 }
 
 }  // namespace bvml_ffn

@@ -8,19 +8,47 @@ namespace bvml_ffn {
 
 namespace {
 
+// 16 bytes of a row from element k on: zeros beyond its end (`end` 0 for no
+// row at all, so that absent rows cost no loads).
+template <int kSize, bool kWhole>
+__device__ __forceinline__ v4i row_piece(const char* at, int k, int end) {
+    constexpr int kPiece = 16 / kSize;
+    v4i v = {0, 0, 0, 0};
+    const int n = end - k;
+    if (n >= kPiece) {
+        __builtin_memcpy(&v, at + (long long)k * kSize, 16);
+    } else if (!kWhole && n > 0) {
+        at = apart(at);
+        if constexpr (kSize == 2) {
+            uint16_t h[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                h[i] = i < n ? reinterpret_cast<const uint16_t*>(at)[k + i] : (uint16_t)0;
+            __builtin_memcpy(&v, h, 16);
+        } else {
+            uint8_t h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                h[i] = i < n ? reinterpret_cast<const uint8_t*>(at)[k + i] : (uint8_t)0;
+            __builtin_memcpy(&v, h, 16);
+        }
+    }
+    return v;
+}
+
 // ---------------------------------------------------------------------------
-// few rows (serving): the weights are read once, by 16 waves a workgroup
-// that share 16 rows of W (gated: 16 of each half) and divide k; their sums
-// meet in LDS.  Bound by reading W: every lane has its 16-byte pieces of
-// kAhead k groups in flight.  The matrix instruction's other operand holds up to 16 rows
-// of x at a time, so a row costs what sixteen cost.
+// few rows (serving): the weights are read once, by workgroups of 8 or 16
+// waves that share 16 rows of W (gated: 16 of each half) and divide k; their
+// sums meet in LDS.  Bound by reading W and, at these sizes, by the latency of
+// doing so: every lane has its 16-byte pieces of kAhead k groups in flight,
+// and what the epilogue adds is asked for first.  The matrix instruction's
+// other operand holds up to 16 rows of x, so a row costs what sixteen cost.
 // ---------------------------------------------------------------------------
-template <int kIn, int kBlocks, bool kGated, bool kWhole>
-__global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product a) {
-    constexpr int kWaves = kBlocks == 4 ? 8 : 16;
+template <int kIn, int kBlocks, int kWaves, bool kGated, bool kWhole>
+__global__ __launch_bounds__(64 * kWaves) void rows_kernel(Product a) {
     constexpr int kHalves = kGated ? 2 : 1;
     constexpr int kSize = kIn == kE4M3 ? 1 : 2, kPiece = 16 / kSize, kStep = 128 / kSize;
-    constexpr int kAhead = kBlocks == 4 ? 1 : 2;
+    constexpr int kAhead = kBlocks == 4 ? 1 : kBlocks == 2 ? 2 : kGated ? 2 : 5;
     __shared__ v4f sums[kWaves][kHalves][kBlocks][64];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -29,12 +57,14 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
     const int row = n0 + i16 < N ? n0 + i16 : N - 1;
     const char* q[kHalves];
     const char* p[kBlocks];
+    int pend[kBlocks];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) q[h] = a.q + (long long)(row + h * N) * a.ldq;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
         const int m = 16 * b + i16;
         p[b] = a.p + (long long)(m < a.M ? m : a.M - 1) * a.ldp;
+        pend[b] = m < a.M ? a.K : 0;
     }
     v4f acc[kHalves][kBlocks];
 #pragma unroll
@@ -42,29 +72,10 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) acc[h][b] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
-    // a lane's piece of k: zeros beyond the row's end
-    auto piece = [&](const char* at, int k) {
-        v4i v = {0, 0, 0, 0};
-        const int n = a.K - k;
-        if (n >= kPiece) {
-            __builtin_memcpy(&v, at + (long long)k * kSize, 16);
-        } else if (!kWhole && n > 0) {
-            if constexpr (kSize == 2) {
-                uint16_t h[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    h[i] = i < n ? reinterpret_cast<const uint16_t*>(at)[k + i] : (uint16_t)0;
-                __builtin_memcpy(&v, h, 16);
-            } else {
-                uint8_t h[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    h[i] = i < n ? reinterpret_cast<const uint8_t*>(at)[k + i] : (uint8_t)0;
-                __builtin_memcpy(&v, h, 16);
-            }
-        }
-        return v;
-    };
+    // wave b finishes rows 16 b .. of x
+    const int type16 = type16_of(kIn, a.e), m = 16 * w + i16, n = n0 + 4 * g;
+    Single<4, kGated> terms;
+    if (w < kBlocks) terms.load(a.e, type16, m, n);
     for (int s = w; s < a.steps; s += kWaves * kAhead) {
         v4i qv[kAhead][kHalves][2], pv[kAhead][kBlocks][2];
 #pragma unroll
@@ -73,9 +84,9 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) qv[u][h][c] = piece(q[h], k + c * 4 * kPiece);
+                for (int h = 0; h < kHalves; ++h) qv[u][h][c] = row_piece<kSize, kWhole>(q[h], k + c * 4 * kPiece, a.K);
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) pv[u][b][c] = piece(p[b], k + c * 4 * kPiece);
+                for (int b = 0; b < kBlocks; ++b) pv[u][b][c] = row_piece<kSize, kWhole>(p[b], k + c * 4 * kPiece, pend[b]);
             }
         }
 #pragma unroll
@@ -102,7 +113,7 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
         for (int b = 0; b < kBlocks; ++b) sums[w][h][b][lane] = acc[h][b];
     __syncthreads();
     if (w >= kBlocks) return;
-    float v[kHalves][4];
+    float v[2][4];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
         v4f t = sums[0][h][w][lane];
@@ -111,41 +122,157 @@ __global__ __launch_bounds__(kBlocks == 4 ? 512 : 1024) void rows_kernel(Product
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[h][r] = t[r];
     }
-    const int m = 16 * w + i16, n = n0 + 4 * g;
-    if constexpr (kGated)
-        finish_one_gated<4>(a.e, type16_of(kIn, a.e), m, n, v[0], v[1]);
-    else
-        finish_one<4>(a.e, type16_of(kIn, a.e), m, n, v[0]);
+    terms.finish(a.e, type16, m, n, v[0], v[1]);
 }
 
-// Sums a split product's parts, in their order, and finishes them.
+// ---------------------------------------------------------------------------
+// one to four rows: a wave takes kRows rows of W (gated: of each half) and the
+// lanes their k, 16 adjacent bytes a lane, so that every load is whole cache
+// lines of one row and the work spreads over every CU.  Products and sums
+// are fp32 on the vector units: at so few rows the weights' way from memory
+// is all that counts.
+// ---------------------------------------------------------------------------
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+// c + the 4 bytes' products
+template <int kIn>
+__device__ __forceinline__ float dot4(int a, int b, float c) {
+    if constexpr (kIn == kBF16) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, a),
+                                               __builtin_bit_cast(v2b, b), c, false);
+    } else if constexpr (kIn == kF16) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, a), __builtin_bit_cast(v2h, b), c,
+                                      false);
+    } else {
+        const v2f a0 = __builtin_amdgcn_cvt_pk_f32_fp8(a, false);
+        const v2f a1 = __builtin_amdgcn_cvt_pk_f32_fp8(a, true);
+        const v2f b0 = __builtin_amdgcn_cvt_pk_f32_fp8(b, false);
+        const v2f b1 = __builtin_amdgcn_cvt_pk_f32_fp8(b, true);
+        c = __builtin_fmaf(a0[0], b0[0], c);
+        c = __builtin_fmaf(a0[1], b0[1], c);
+        c = __builtin_fmaf(a1[0], b1[0], c);
+        return __builtin_fmaf(a1[1], b1[1], c);
+    }
+}
+
+// The wave's sum, to every lane: within rows of 16 lanes, then across them.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                             0, __builtin_bit_cast(int, v), kCtrl, kRowMask, 0xf,
+                                             kRowMask == 0xf));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);  // row_bcast 15 to rows 1 and 3
+    v = dpp_add<0x143, 0xc>(v);  // row_bcast 31 to rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+template <int kIn, int kM, int kRows, bool kGated, bool kWhole>
+__global__ __launch_bounds__(256) void dot_kernel(Product a) {
+    constexpr int kHalves = kGated ? 2 : 1;
+    constexpr int kSize = kIn == kE4M3 ? 1 : 2, kPiece = 16 / kSize;
+    constexpr int kAhead = kM * kHalves * kRows >= 8 ? 3 : 5;
+    const int lane = threadIdx.x & 63;
+    const int N = a.e.N, n0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows;
+    if (n0 >= N) return;
+    const char* q[kHalves][kRows];
+    const char* p[kM];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+            q[h][r] = a.q + (long long)((n0 + r < N ? n0 + r : N - 1) + h * N) * a.ldq;
+#pragma unroll
+    for (int m = 0; m < kM; ++m) p[m] = a.p + (long long)(m < a.M ? m : a.M - 1) * a.ldp;
+    // lane m kRows + r finishes row m, column n0 + r
+    const int type16 = type16_of(kIn, a.e), mine = lane / kRows, n = n0 + lane % kRows;
+    Single<1, kGated> terms;
+    if (mine < kM) terms.load(a.e, type16, mine, n);
+    float acc[kHalves][kM][kRows];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) acc[h][m][r] = 0.0f;
+
+    for (int k0 = lane * kPiece; k0 < a.K; k0 += 64 * kPiece * kAhead) {
+        v4i qv[kAhead][kHalves][kRows], pv[kAhead][kM];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = k0 + u * 64 * kPiece;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int r = 0; r < kRows; ++r)
+                    qv[u][h][r] = row_piece<kSize, kWhole>(q[h][r], k, a.K);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) pv[u][m] = row_piece<kSize, kWhole>(p[m], k, a.K);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int m = 0; m < kM; ++m)
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[h][m][r] = dot4<kIn>(qv[u][h][r][i], pv[u][m][i], acc[h][m][r]);
+    }
+    float v[1] = {0.0f}, w[1] = {0.0f};
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const float t = wave_sum(acc[h][m][r]);
+                if (lane == m * kRows + r) (h ? w : v)[0] = t;
+            }
+    if (mine < kM) terms.finish(a.e, type16, mine, n, v, w);
+}
+
+// Sums the parts of the split tiles, in their order, and finishes them: a
+// thread 8 columns of a row, blockIdx.y the tile.
 template <bool kGated>
-__global__ __launch_bounds__(256) void join_kernel(Epilogue e, int in_type, int splits) {
-    const int per = (e.N + 3) / 4;
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long m = t / per;
-    if (m >= e.M) return;
-    const int n = (int)(t % per) * 4, c = e.N - n;
-    const int R = kGated ? 2 * e.N : e.N;
-    float v[4], u[4];
+__global__ __launch_bounds__(256) void join_kernel(Product a, int in_type, int bm, int bn) {
+    const int cols = kGated ? bn / 2 : bn, per = cols / 8;
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    const int row = t / per, col = t % per * 8;
+    if (row >= bm) return;
+    int tm, tn;
+    tile_of(a.whole + blockIdx.y, a.tiles_m, a.tiles_n, tm, tn);
+    const int m = tm * bm + row, n = tn * cols + col;
+    if (m >= a.M || n >= a.e.N) return;
+    const float* from = a.e.part + (long long)blockIdx.y * a.splits * bm * bn + row * bn + col;
+    const int type16 = type16_of(in_type, a.e);
+    Single<8, kGated> terms;
+    terms.load(a.e, type16, m, n);
+    float v[8], u[8];
+    load_row<8>(from, kF32, 0, 8, v);
+    if constexpr (kGated) load_row<8>(from, kF32, cols, 8, u);
+    for (int s = 1; s < a.splits; ++s) {
+        from += bm * bn;
+        float x[8];
+        load_row<8>(from, kF32, 0, 8, x);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = u[r] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-        const long long at = ((long long)s * e.M + m) * R + n;
-        float x[4];
-        load_row<4>(e.part, kF32, at, c, x);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += x[r];
+        for (int i = 0; i < 8; ++i) v[i] += x[i];
         if constexpr (kGated) {
-            load_row<4>(e.part, kF32, at + e.N, c, x);
+            load_row<8>(from, kF32, cols, 8, x);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) u[r] += x[r];
+            for (int i = 0; i < 8; ++i) u[i] += x[i];
         }
     }
-    if constexpr (kGated)
-        finish_one_gated<4>(e, type16_of(in_type, e), (int)m, n, v, u);
-    else
-        finish_one<4>(e, type16_of(in_type, e), (int)m, n, v);
+    terms.finish(a.e, type16, m, n, v, u);
 }
 
 int step_of(int in_type) { return in_type == kE4M3 ? 128 : 64; }
@@ -164,31 +291,52 @@ Product product_of(const ProductCall& c) {
     a.R = c.R;
     a.tiles_m = a.tiles_n = 0;
     a.steps = (int)ceil_div(c.K, step_of(c.in_type));
+    a.whole = 0;
+    a.splits = 1;
     a.per_split = a.steps;
     a.e = c.e;
     return a;
 }
 
+template <int kIn, int kBlocks, int kWaves, bool kGated>
+hipError_t launch_rows_one(const Product& a, bool whole, hipStream_t s) {
+    const dim3 grid((unsigned)((a.e.N + 15) / 16)), block(64 * kWaves);
+    if (whole)
+        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kWaves, kGated, true>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kWaves, kGated, false>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
+template <int kIn, int kM, int kRows, bool kGated>
+hipError_t launch_dot_one(const Product& a, bool whole, hipStream_t s) {
+    const dim3 grid((unsigned)((a.e.N + 4 * kRows - 1) / (4 * kRows))), block(256);
+    if (whole)
+        hipLaunchKernelGGL((dot_kernel<kIn, kM, kRows, kGated, true>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((dot_kernel<kIn, kM, kRows, kGated, false>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
+template <int kIn, int kM, bool kGated>
+hipError_t launch_dot_of(const Product& a, bool whole, hipStream_t s) {
+    // two columns a wave once that leaves two workgroups a CU
+    return a.e.N >= 4096 ? launch_dot_one<kIn, kM, 2, kGated>(a, whole, s)
+                         : launch_dot_one<kIn, kM, 1, kGated>(a, whole, s);
+}
+
 template <int kIn, bool kGated>
 hipError_t launch_rows_of(const Product& a, bool whole, hipStream_t s) {
-    const int blocks = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    const dim3 grid((unsigned)((a.e.N + 15) / 16));
-#define BVML_FFN_ROWS(B)                                                                     \
-    if (whole)                                                                               \
-        hipLaunchKernelGGL((rows_kernel<kIn, B, kGated, true>), grid, dim3(B == 4 ? 512 : 1024), \
-                           0, s, a);                                                         \
-    else                                                                                     \
-        hipLaunchKernelGGL((rows_kernel<kIn, B, kGated, false>), grid,                       \
-                           dim3(B == 4 ? 512 : 1024), 0, s, a);
-    if (blocks == 1) {
-        BVML_FFN_ROWS(1)
-    } else if (blocks == 2) {
-        BVML_FFN_ROWS(2)
-    } else {
-        BVML_FFN_ROWS(4)
-    }
-#undef BVML_FFN_ROWS
-    return hipGetLastError();
+    if (a.M == 1) return launch_dot_of<kIn, 1, kGated>(a, whole, s);
+    if (a.M == 2) return launch_dot_of<kIn, 2, kGated>(a, whole, s);
+    if (a.M <= 4) return launch_dot_of<kIn, 4, kGated>(a, whole, s);
+    // 16 waves where the workgroups are few and k is long enough for them
+    const bool wide = a.e.N <= 16 * 256 && a.steps >= 32;
+    if (a.M <= 16)
+        return wide ? launch_rows_one<kIn, 1, 16, kGated>(a, whole, s)
+                    : launch_rows_one<kIn, 1, 8, kGated>(a, whole, s);
+    if (a.M <= 32) return launch_rows_one<kIn, 2, 8, kGated>(a, whole, s);
+    return launch_rows_one<kIn, 4, 8, kGated>(a, whole, s);
 }
 
 hipError_t launch_rows(const ProductCall& c, hipStream_t s) {
@@ -215,51 +363,262 @@ bool dma_fits(const ProductCall& c) {
     return (along % piece == 0 || c.padded_p) && c.R % piece == 0;
 }
 
+namespace {
+
+// What a tile costs, in us, measured on bf16 products of 1,280 to 8,192 terms:
+// `fixed` for its first copies and its epilogue, `step` for 128 bytes of k with
+// the card full and `idle` with one workgroup on half of the CUs at most.
+// `room`: workgroups on the card at once.
+// `across`: what an operand read across its rows adds to a step.
+struct TileCost {
+    int bm, bn, room;
+    double fixed, step, idle, across;
+};
+constexpr TileCost kCosts[] = {
+    {256, 256, 256, 9.0, 1.42, 1.03, 0.06},  // 4096^2 x 8192 at 1350 TFLOP/s
+    {128, 128, 512, 5.0, 0.87, 0.65, 0.12},  // 1130
+    {128, 128, 256, 4.0, 0.47, 0.45, 0.12},  // 2048^2 x 5120: 45 us, 59 with two slots
+    {64, 128, 512, 3.0, 0.55, 0.33, 0.12},   // 2048 x 1024 x 5120: 30 us
+};
+// A second launch, and a byte of a part written and read.
+constexpr double kJoin = 5.0, kJoinBytes = 8.0 / 4e6;
+
+}  // namespace
+
 ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
-    ProductPlan p{kTileRows, dma, 1};
-    if (layout == kForward && M <= 64) return p;
+    if (layout == kForward && M <= 64) return {kTileRows, dma, 0, 1};
     const int n = gated ? R / 2 : R;
-    auto tiles = [&](int b) { return ceil_div(M, b) * ceil_div(n, gated ? b / 2 : b); };
     const long long steps = ceil_div(K, step_of(in_type));
-    p.tile = !dma ? kTile128 : tiles(256) >= 160 ? kTile256 : tiles(128) >= 128 ? kTile128 : kTile64;
-    const int b = p.tile == kTile256 ? 256 : p.tile == kTile128 ? 128 : 64;
-    const long long room = p.tile == kTile256 ? 256 : 512;
-    if (tiles(b) > 0 && tiles(b) * 2 <= room) {
-        long long s = room / tiles(b);
-        if (s > steps / 4) s = steps / 4;
-        if (s > 16) s = 16;
-        if (s > 1) p.splits = (int)ceil_div(steps, ceil_div(steps, s));
+    ProductPlan best{kTile128, dma, 0, 1};
+    double least = 1e30;
+    for (int tile = kTile256; tile <= kTile64; ++tile) {
+        if (!dma && tile != kTile128) continue;
+        const TileCost& c = kCosts[tile];
+        const long long tiles = ceil_div(M, c.bm) * ceil_div(n, gated ? c.bn / 2 : c.bn);
+        // rounds of a full card, then what is left over: one workgroup a tile
+        // or, where that leaves CUs idle, several that share its terms
+        const long long left = tiles % c.room;
+        const double slower = 1.0 + layout * c.across;
+        const double rounds = (double)(tiles / c.room) * (c.fixed + steps * c.step * slower);
+        for (int s = 1; s <= 64; ++s) {
+            if (s > 1 && (left * s > c.room || steps < 4 * s)) break;
+            const long long each = ceil_div(steps, s);
+            if (s > 1 && ceil_div(steps, each) != s) continue;  // a part with nothing
+            double t = rounds;
+            if (left > 0) {
+                const double full = (double)(left * s) / c.room;
+                const double step = full <= 0.5 ? c.idle : c.idle + (c.step - c.idle) * (2 * full - 1);
+                t += c.fixed + each * step * slower;
+            }
+            if (s > 1) t += kJoin + (double)(left * s) * c.bm * c.bn * kJoinBytes;
+            if (t < least) {
+                least = t;
+                best = {tile, dma, (int)(s > 1 ? tiles - left : tiles), s};
+            }
+        }
     }
-    return p;
+    return best;
 }
 
+namespace {
+long long parts_of(int M, int R, bool gated, const ProductPlan& p) {
+    if (p.tile == kTileRows || p.splits == 1) return 0;
+    const TileCost& c = kCosts[p.tile];
+    const int n = gated ? R / 2 : R;
+    return ceil_div(M, c.bm) * ceil_div(n, gated ? c.bn / 2 : c.bn) - p.whole;
+}
+}  // namespace
+
 long long product_workspace(int M, int R, int K, int in_type, int layout, bool gated) {
-    int splits = 1;
+    long long most = 0;
     for (const bool dma : {false, true}) {
         const ProductPlan p = plan_product(M, R, K, in_type, layout, gated, dma);
-        if (p.splits > splits) splits = p.splits;
+        const long long parts = parts_of(M, R, gated, p) * p.splits;
+        if (parts == 0) continue;
+        const long long bytes = parts * kCosts[p.tile].bm * kCosts[p.tile].bn * 4;
+        if (bytes > most) most = bytes;
     }
-    return splits > 1 ? (long long)splits * M * R * 4 : 0;
+    return most;
 }
+
+namespace {
+
+// A product's tiles as the plan has them.
+void lay_out(Product& a, const ProductCall& c, int tile, int whole, int splits, void* workspace) {
+    const TileCost& t = kCosts[tile];
+    a.tiles_m = (int)ceil_div(c.M, t.bm);
+    a.tiles_n = (int)ceil_div(c.gated ? c.R / 2 : c.R, c.gated ? t.bn / 2 : t.bn);
+    a.whole = whole;
+    a.splits = splits;
+    a.per_split = (int)ceil_div(a.steps, splits);
+    a.e.part = static_cast<float*>(workspace);
+}
+
+hipError_t join(const Product& a, const ProductCall& c, int tile, hipStream_t s) {
+    const long long parts = (long long)a.tiles_m * a.tiles_n - a.whole;
+    if (parts == 0) return hipSuccess;
+    const TileCost& t = kCosts[tile];
+    const int cols = c.gated ? t.bn / 2 : t.bn;
+    const dim3 grid((unsigned)ceil_div(t.bm * cols / 8, 256), (unsigned)parts);
+    if (c.gated)
+        hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, s, a, c.in_type, t.bm, t.bn);
+    else
+        hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, s, a, c.in_type, t.bm, t.bn);
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s) {
     const ProductPlan p =
         plan_product(c.M, c.R, c.K, c.in_type, c.layout, c.gated, dma_fits(c));
     if (p.tile == kTileRows) return launch_rows(c, s);
     Product a = product_of(c);
-    a.per_split = (int)ceil_div(a.steps, p.splits);
-    if (p.splits > 1) a.e.part = static_cast<float*>(workspace);
-    hipError_t err = c.in_type == kF16    ? launch_tiles_f16(a, p, c.layout, c.gated, s)
-                     : c.in_type == kBF16 ? launch_tiles_bf16(a, p, c.layout, c.gated, s)
-                                          : launch_tiles_e4m3(a, p, c.layout, c.gated, s);
-    if (err != hipSuccess || p.splits == 1) return err;
-    const long long threads = (long long)c.M * ((a.e.N + 3) / 4);
-    const dim3 grid((unsigned)ceil_div(threads, 256));
-    if (c.gated)
-        hipLaunchKernelGGL(join_kernel<true>, grid, dim3(256), 0, s, a.e, c.in_type, p.splits);
-    else
-        hipLaunchKernelGGL(join_kernel<false>, grid, dim3(256), 0, s, a.e, c.in_type, p.splits);
-    return hipGetLastError();
+    lay_out(a, c, p.tile, p.whole, p.splits, workspace);
+    if ((long long)a.tiles_m * a.tiles_n > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    const hipError_t e = c.in_type == kF16    ? launch_tiles_f16(a, p, c.layout, c.gated, s)
+                         : c.in_type == kBF16 ? launch_tiles_bf16(a, p, c.layout, c.gated, s)
+                                              : launch_tiles_e4m3(a, p, c.layout, c.gated, s);
+    return e == hipSuccess ? join(a, c, p.tile, s) : e;
+}
+
+namespace {
+
+// When n1 jobs of t1 and then n2 of t2 <= t1 are done on `room` slots, each
+// slot taking the next job as it comes free.
+double done_by(long long n1, double t1, long long n2, double t2, int room) {
+    const long long a = n1 / room, over = n1 % room;
+    const double early = a * t1, late = over > 0 ? early + t1 : early;
+    // room - over slots come free at `early`, the others at `late`; what fits by T
+    auto fit = [&](double T) {
+        const double x = (T - early) / t2 + 1e-9, y = (T - early - t1) / t2 + 1e-9;
+        return (room - over) * (x > 0 ? (long long)x : 0) + over * (y > 0 ? (long long)y : 0);
+    };
+    if (fit(late) >= n2) return late;
+    // T one job after a slot of either kind came free
+    double best = 1e30;
+    for (int kind = 0; kind < (over > 0 ? 2 : 1); ++kind) {
+        const double from = kind == 0 ? early : early + t1;
+        long long lo = 0, hi = n2 / (over > 0 && kind == 1 ? over : room - over) + 1;
+        while (lo < hi) {
+            const long long k = (lo + hi) / 2;
+            if (fit(from + k * t2) >= n2) hi = k;
+            else lo = k + 1;
+        }
+        const double T = from + lo * t2;
+        if (T < best) best = T;
+    }
+    return best > late ? best : late;
+}
+
+GradientsPlan search_gradients(int M, int R, int K) {
+    static const int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    GradientsPlan best{kTile128, false, 0, 1, 0, 1};
+    double least = 1e30;
+    const long long si = ceil_div(R, 64), sw = ceil_div(M, 64);  // steps of a tile
+    for (int tile = kTile256; tile <= kTile64; ++tile) {
+        const TileCost& c = kCosts[tile];
+        const double bytes = (double)c.bm * c.bn * kJoinBytes;
+        const long long cols = ceil_div(K, c.bn);
+        const long long ti = ceil_div(M, c.bm) * cols, tw = ceil_div(R, c.bm) * cols;
+        auto time = [&](long long steps, int across) {
+            return c.fixed + steps * c.step * (1.0 + across * c.across);
+        };
+        auto may = [&](long long tiles, long long steps, int s) {
+            return s == 1 || (steps >= 4 * s && ceil_div(steps, ceil_div(steps, s)) == s &&
+                              tiles * s <= 2 * c.room);
+        };
+        // every tile of a product in s parts
+        for (const int a : kSplits) {
+            if (!may(ti, si, a)) continue;
+            for (const int b : kSplits) {
+                if (!may(tw, sw, b)) continue;
+                const double x = time(ceil_div(si, a), 1), w = time(ceil_div(sw, b), 2);
+                double t = w > x ? done_by(tw * b, w, ti * a, x, c.room)
+                                 : done_by(ti * a, x, tw * b, w, c.room);
+                if (a > 1) t += kJoin + ti * a * bytes;
+                if (b > 1) t += kJoin + tw * b * bytes;
+                if (t < least) {
+                    least = t;
+                    best = {tile, w > x, a > 1 ? 0 : (int)ti, a, b > 1 ? 0 : (int)tw, b};
+                }
+            }
+        }
+        // or the shorter product's last tiles, those beyond whole rounds
+        const double x = time(si, 1), w = time(sw, 2);
+        const bool first = w > x;
+        const long long longs = first ? tw : ti, shorts = first ? ti : tw;
+        const long long steps = first ? si : sw;
+        for (long long rest = 1; rest < shorts && rest <= c.room / 2; rest += rest < 8 ? 1 : rest / 4) {
+            const double t0 = done_by(longs, first ? w : x, shorts - rest, first ? x : w, c.room);
+            if (t0 >= least) continue;
+            for (const int s : kSplits) {
+                if (s == 1 || !may(rest, steps, s)) continue;
+                const double one = time(ceil_div(steps, s), first ? 1 : 2);
+                const double t = t0 + one * ceil_div(rest * s, c.room) + kJoin + rest * s * bytes;
+                if (t < least) {
+                    least = t;
+                    best = first ? GradientsPlan{tile, true, (int)(ti - rest), s, (int)tw, 1}
+                                 : GradientsPlan{tile, false, (int)ti, 1, (int)(tw - rest), s};
+                }
+            }
+        }
+    }
+    return best;
+}
+
+}  // namespace
+
+// (The search takes some tens of microseconds: a thread keeps its last plans,
+// by their sizes.)
+GradientsPlan plan_gradients(int M, int R, int K) {
+    struct Known {
+        int M, R, K;
+        GradientsPlan plan;
+    };
+    thread_local Known known[64] = {};
+    Known& k = known[((unsigned)M * 31u + (unsigned)R * 17u + (unsigned)K) % 64u];
+    if (k.M != M || k.R != R || k.K != K) k = {M, R, K, search_gradients(M, R, K)};
+    return k.plan;
+}
+
+namespace {
+long long part_bytes(long long tiles, int whole, int splits, int tile) {
+    return splits == 1 ? 0 : (tiles - whole) * splits * kCosts[tile].bm * kCosts[tile].bn * 4;
+}
+}  // namespace
+
+long long gradients_workspace(int M, int R, int K) {
+    if (M == 0) return 0;
+    const GradientsPlan p = plan_gradients(M, R, K);
+    const TileCost& c = kCosts[p.tile];
+    const long long cols = ceil_div(K, c.bn);
+    return part_bytes(ceil_div(M, c.bm) * cols, p.input_whole, p.input_splits, p.tile) +
+           part_bytes(ceil_div(R, c.bm) * cols, p.weight_whole, p.weight_splits, p.tile);
+}
+
+hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight, void* workspace,
+                            hipStream_t s) {
+    if (input.M == 0 || !dma_fits(input) || !dma_fits(weight)) {
+        if (input.M > 0) {
+            const hipError_t e = launch_product(input, workspace, s);
+            if (e != hipSuccess) return e;
+        }
+        return launch_product(weight, workspace, s);
+    }
+    const GradientsPlan p = plan_gradients(input.M, input.K, input.R);
+    Gradients g{product_of(input), product_of(weight), p.weight_first};
+    lay_out(g.input, input, p.tile, p.input_whole, p.input_splits, workspace);
+    const long long ti = (long long)g.input.tiles_m * g.input.tiles_n;
+    lay_out(g.weight, weight, p.tile, p.weight_whole, p.weight_splits,
+            static_cast<char*>(workspace) + part_bytes(ti, p.input_whole, p.input_splits, p.tile));
+    if (ti > 0x7fffffffLL || (long long)g.weight.tiles_m * g.weight.tiles_n > 0x7fffffffLL)
+        return hipErrorInvalidConfiguration;
+    hipError_t e = input.in_type == kF16 ? launch_gradients_f16(g, p.tile, s)
+                                         : launch_gradients_bf16(g, p.tile, s);
+    if (e == hipSuccess) e = join(g.input, input, p.tile, s);
+    if (e == hipSuccess) e = join(g.weight, weight, p.tile, s);
+    return e;
 }
 
 }  // namespace bvml_ffn

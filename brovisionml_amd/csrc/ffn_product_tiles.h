@@ -3,31 +3,52 @@
 // a translation unit each so that they compile side by side.
 #pragma once
 
+#include <initializer_list>
+
 #include "ffn_kernels.h"
 #include "ffn_product.h"
 
 namespace bvml_ffn {
 
-template <int kIn, int BM, int BN, int WM, int WN, bool PT, bool QT, bool G, bool D>
-hipError_t launch_one(const Product& a, int splits, hipStream_t s) {
-    Product c = a;
-    const int cols = G ? BN / 2 : BN;
-    c.tiles_m = (a.M + BM - 1) / BM;
-    c.tiles_n = ((G ? a.R / 2 : a.R) + cols - 1) / cols;
-    const long long tiles = (long long)c.tiles_m * c.tiles_n;
-    if (tiles > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((product_kernel<kIn, BM, BN, WM, WN, PT, QT, G, D>),
-                       dim3((unsigned)tiles, (unsigned)splits), dim3(64 * WM * WN), 0, s, c);
+template <int kIn, int BM, int BN, int S, bool PT, bool QT, bool G, bool D>
+hipError_t launch_one(const Product& a, hipStream_t s) {
+    const long long rest = (long long)a.tiles_m * a.tiles_n - a.whole;
+    const long long groups = a.whole + rest * a.splits;
+    if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((product_kernel<kIn, BM, BN, S, PT, QT, G, D>), dim3((unsigned)groups),
+                       dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 template <int kIn, bool PT, bool QT, bool G>
 hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) {
-    if (!p.dma) return launch_one<kIn, 128, 128, 2, 2, PT, QT, G, false>(a, p.splits, s);
+    if (!p.dma) return launch_one<kIn, 128, 128, 2, PT, QT, G, false>(a, s);
     switch (p.tile) {
-        case kTile256: return launch_one<kIn, 256, 256, 2, 2, PT, QT, G, true>(a, p.splits, s);
-        case kTile128: return launch_one<kIn, 128, 128, 2, 2, PT, QT, G, true>(a, p.splits, s);
-        default: return launch_one<kIn, 64, 128, 2, 2, PT, QT, G, true>(a, p.splits, s);
+        case kTile256: return launch_one<kIn, 256, 256, 2, PT, QT, G, true>(a, s);
+        case kTile128: return launch_one<kIn, 128, 128, 2, PT, QT, G, true>(a, s);
+        case kTile128Deep: return launch_one<kIn, 128, 128, 4, PT, QT, G, true>(a, s);
+        default: return launch_one<kIn, 64, 128, 3, PT, QT, G, true>(a, s);
+    }
+}
+
+template <int kIn, int BM, int BN, int S>
+hipError_t launch_both(const Gradients& g, hipStream_t s) {
+    long long groups = 0;
+    for (const Product* a : {&g.input, &g.weight})
+        groups += a->whole + ((long long)a->tiles_m * a->tiles_n - a->whole) * a->splits;
+    if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((gradients_kernel<kIn, BM, BN, S>), dim3((unsigned)groups), dim3(256), 0, s,
+                       g);
+    return hipGetLastError();
+}
+
+template <int kIn>
+hipError_t launch_gradient_tiles(const Gradients& g, int tile, hipStream_t s) {
+    switch (tile) {
+        case kTile256: return launch_both<kIn, 256, 256, 2>(g, s);
+        case kTile128: return launch_both<kIn, 128, 128, 2>(g, s);
+        case kTile128Deep: return launch_both<kIn, 128, 128, 4>(g, s);
+        default: return launch_both<kIn, 64, 128, 3>(g, s);
     }
 }
 

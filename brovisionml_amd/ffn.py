@@ -26,7 +26,6 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .dsine import _launch
 
 _WHO = "ffn ops: "
 _TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16,
@@ -52,21 +51,25 @@ def _fail(msg: str):
     raise RuntimeError(_WHO + msg)
 
 
-def _raise_status(op: str, status: int) -> None:
-    if status != _lib.OK:
-        _fail(f"{op}: {_lib.ffn_last_error()} (status {status})")
+# The checks below take the cheapest queries for the usual call: at a few rows
+# the kernels take less time than they do.
+_VALUES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_HALVES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_OPERANDS = {**_HALVES, torch.float8_e4m3fn: _lib.E4M3}
+_F32 = torch.float32
 
 
 def _rows(op: str, name: str, t):
     """(rows, columns, elements from row to row) of a tensor whose leading
     dimensions collapse to evenly spaced rows."""
     shape, stride = t.shape, t.stride()
-    if not shape:
-        _fail(f"{op}: {name} must have at least one dimension")
-    cols = shape[-1]
     if len(shape) == 2:
-        rows, step = shape[0], stride[0]
+        rows, cols = shape
+        step = stride[0]
+    elif not shape:
+        _fail(f"{op}: {name} must have at least one dimension")
     else:
+        cols = shape[-1]
         rows, step = 1, cols
         for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
             if n == 1:
@@ -82,50 +85,60 @@ def _rows(op: str, name: str, t):
     return rows, cols, (step if rows > 1 else cols)
 
 
-def _check(op: str, first, **tensors) -> None:
-    """Every tensor on one HIP device."""
-    if not first.is_cuda:
+def _index(op: str, t) -> int:
+    if not t.is_cuda:
         _fail(f"{op}: tensors must be on a HIP device")
-    index = first.get_device()
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != index:
-            _fail(f"{op}: {name} must be on the same device as the others")
+    return t.get_device()
 
 
 def _type(op: str, name: str, dtype, allowed) -> int:
-    if dtype not in allowed:
-        _fail(f"{op}: {name} is {dtype}, expected one of "
-              + ", ".join(str(d) for d in allowed))
-    return _TYPES[dtype]
+    kind = allowed.get(dtype)
+    if kind is None:
+        _fail(f"{op}: {name} is {dtype}, expected one of " + ", ".join(str(d) for d in allowed))
+    return kind
 
 
-def _vector(op: str, name: str, t, n: int, allowed):
-    """(address, type) of a contiguous vector of n, (0, F32) for None."""
-    if t is None:
-        return 0, _lib.F32
-    kind = _type(op, name, t.dtype, allowed)
+def _vector(op: str, name: str, t, index: int, n: int, *allowed):
+    """(address, type) of a contiguous vector of n on the operands' device."""
+    if t.dtype not in allowed:
+        _fail(f"{op}: {name} is {t.dtype}, expected one of " + ", ".join(str(d) for d in allowed))
     if t.numel() != n or not t.is_contiguous():
         _fail(f"{op}: {name} must be a contiguous tensor of {n} elements, got {tuple(t.shape)}")
-    return t.data_ptr(), kind
+    if t.get_device() != index:
+        _fail(f"{op}: {name} must be on the same device as the others")
+    return t.data_ptr(), _TYPES[t.dtype]
 
 
-_VALUES = (torch.float32, torch.float16, torch.bfloat16)
-_HALVES = (torch.float16, torch.bfloat16)
-_F32 = (torch.float32,)
-
-
-def _same(op: str, name: str, t, shape, dtype):
-    """Row step of t, which must have this shape and type."""
+def _same(op: str, name: str, t, index: int, shape, dtype):
+    """(address, row step) of t, which must have this shape, type and device."""
     if t.shape != shape:
         _fail(f"{op}: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         _fail(f"{op}: {name} is {t.dtype}, expected {dtype}")
-    return _rows(op, name, t)[2]
+    if t.get_device() != index:
+        _fail(f"{op}: {name} must be on the same device as the others")
+    return t.data_ptr(), _rows(op, name, t)[2]
+
+
+def _launch(op: str, index: int, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of device `index`, with that
+    device current; raises on a refusal."""
+    if _device() == index:
+        status = fn(*args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _stream(index))
+    if status != _lib.OK:
+        _fail(f"{op}: {_lib.ffn_last_error()} (status {status})")
+
+
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _space(n: int, like):
     """n bytes of workspace on like's device (None for none) and its address."""
-    if n == 0:
+    if n <= 0:
         return None, 0
     t = torch.empty(n, dtype=torch.uint8, device=like.device)
     return t, t.data_ptr()
@@ -143,23 +156,31 @@ def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, *, dtype=None
     with save, the rows' rstd for the backward pass.  The weight is float32
     or of x's type; None means ones."""
     op = "add_rms_norm"
-    _check(op, x, residual=residual, weight=weight)
-    xt = _type(op, "x", x.dtype, _VALUES)
+    index, xd = _index(op, x), x.dtype
+    xt = _type(op, "x", xd, _VALUES)
     rows, cols, ldx = _rows(op, "x", x)
-    ldr = 0 if residual is None else _same(op, "residual", residual, x.shape, x.dtype)
-    wp, wt = _vector(op, "weight", weight, cols, (torch.float32, x.dtype))
-    dtype = x.dtype if dtype is None else dtype
-    yt = _TYPES.get(dtype, -1)
-    y = torch.empty(x.shape, dtype=dtype, device=x.device)
-    lead = x.shape[:-1]
-    scale = torch.empty(lead, dtype=torch.float32, device=x.device) if yt == _lib.E4M3 else None
-    rstd = torch.empty(lead, dtype=torch.float32, device=x.device) if save else None
-    stream = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    st = _launch(x, _lib.load_ffn().bvml_ffn_add_rms_norm, x.data_ptr(), ldx,
-                 0 if residual is None else residual.data_ptr(), ldr, wp, rows, cols, eps, xt, wt,
-                 yt, y.data_ptr(), cols, 0 if residual is None else stream.data_ptr(), cols,
-                 0 if scale is None else scale.data_ptr(), 0 if rstd is None else rstd.data_ptr())
-    _raise_status(op, st)
+    shape = x.shape
+    wp = wt = rp = ldr = sp = cp = dp = 0
+    scale = rstd = None
+    stream = x
+    if weight is not None:
+        wp, wt = _vector(op, "weight", weight, index, cols, _F32, xd)
+    if residual is not None:
+        rp, ldr = _same(op, "residual", residual, index, shape, xd)
+        stream = x.new_empty(shape)
+        sp = stream.data_ptr()
+    if dtype is None or dtype == xd:
+        yt, y = xt, x.new_empty(shape)
+    else:
+        yt, y = _TYPES.get(dtype, -1), x.new_empty(shape, dtype=dtype)
+        if yt == _lib.E4M3:
+            scale = x.new_empty(shape[:-1], dtype=_F32)
+            cp = scale.data_ptr()
+    if save:
+        rstd = x.new_empty(shape[:-1], dtype=_F32)
+        dp = rstd.data_ptr()
+    _launch(op, index, _lib.load_ffn().bvml_ffn_add_rms_norm, x.data_ptr(), ldx, rp, ldr, wp, rows,
+            cols, eps, xt, wt, yt, y.data_ptr(), cols, sp, cols, cp, dp)
     return Norm(y, scale, stream, rstd)
 
 
@@ -168,24 +189,27 @@ def add_rms_norm_backward(dy, stream, weight, rstd, dstream=None, *, need_weight
     weight's, from dy, the forward pass's stream and rstd, and the gradient
     that reaches the stream itself."""
     op = "add_rms_norm_backward"
-    _check(op, stream, dy=dy, weight=weight, rstd=rstd, dstream=dstream)
-    st_t = _type(op, "stream", stream.dtype, _VALUES)
+    index, sd = _index(op, stream), stream.dtype
+    st = _type(op, "stream", sd, _VALUES)
     dt = _type(op, "dy", dy.dtype, _VALUES)
     rows, cols, lds = _rows(op, "stream", stream)
-    lddy = _same(op, "dy", dy, stream.shape, dy.dtype)
-    lddst = 0 if dstream is None else _same(op, "dstream", dstream, stream.shape, stream.dtype)
-    wp, wt = _vector(op, "weight", weight, cols, (torch.float32, stream.dtype))
-    rp, _ = _vector(op, "rstd", rstd, rows, _F32)
-    ds = torch.empty(stream.shape, dtype=stream.dtype, device=stream.device)
-    dw = torch.empty_like(weight) if weight is not None and need_weight else None
+    yp, lddy = _same(op, "dy", dy, index, stream.shape, dy.dtype)
+    rp, _ = _vector(op, "rstd", rstd, index, rows, _F32)
+    wp = wt = gp = ldg = dwp = n = 0
+    dw = None
     lib = _lib.load_ffn()
-    n = lib.bvml_ffn_add_rms_norm_backward_workspace(rows, cols) if dw is not None else 0
-    space, sp = _space(max(n, 0), stream)
-    st = _launch(stream, lib.bvml_ffn_add_rms_norm_backward, dy.data_ptr(), lddy,
-                 stream.data_ptr(), lds, wp, rp, 0 if dstream is None else dstream.data_ptr(),
-                 lddst, rows, cols, dt, st_t, wt, ds.data_ptr(), cols,
-                 0 if dw is None else dw.data_ptr(), sp, n)
-    _raise_status(op, st)
+    if weight is not None:
+        wp, wt = _vector(op, "weight", weight, index, cols, _F32, sd)
+        if need_weight:
+            dw = torch.empty_like(weight)
+            dwp = dw.data_ptr()
+            n = lib.bvml_ffn_add_rms_norm_backward_workspace(rows, cols)
+    if dstream is not None:
+        gp, ldg = _same(op, "dstream", dstream, index, stream.shape, sd)
+    ds = stream.new_empty(stream.shape)
+    space, sp = _space(n, stream)
+    _launch(op, index, lib.bvml_ffn_add_rms_norm_backward, yp, lddy, stream.data_ptr(), lds, wp, rp,
+            gp, ldg, rows, cols, dt, st, wt, ds.data_ptr(), cols, dwp, sp, n)
     return ds, dw
 
 
@@ -206,54 +230,57 @@ def _backward_space(gated: bool, M: int, N: int, K: int) -> int:
 
 
 def _forward(op: str, gated: bool, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out):
-    _check(op, x, w=w, bias=bias, residual=residual, x_scale=x_scale, w_scale=w_scale, out=out)
-    kind = _type(op, "x", x.dtype, (*_HALVES, torch.float8_e4m3fn))
-    if w.dtype != x.dtype:
-        _fail(f"{op}: w is {w.dtype}, x {x.dtype}: one type for both")
+    index, xd = _index(op, x), x.dtype
+    kind = _type(op, "x", xd, _OPERANDS)
+    if w.dtype != xd:
+        _fail(f"{op}: w is {w.dtype}, x {xd}: one type for both")
     if w.dim() != 2:
         _fail(f"{op}: w must have two dimensions")
+    if w.get_device() != index:
+        _fail(f"{op}: w must be on the same device as the others")
     M, K, ldx = _rows(op, "x", x)
     R, Kw, ldw = _rows(op, "w", w)
     if Kw != K:
         _fail(f"{op}: w has rows of {Kw}, x of {K}")
-    if gated and R % 2:
-        _fail(f"{op}: w must stack the gate's and the other half's rows: {R} is odd")
-    N = R // 2 if gated else R
-    if act not in _ACTS:
+    N = R
+    if gated:
+        if R % 2:
+            _fail(f"{op}: w must stack the gate's and the other half's rows: {R} is odd")
+        N = R // 2
+    code = _ACTS.get(act)
+    if code is None:
         _fail(f"{op}: unknown activation {act!r}, expected one of " + ", ".join(_ACTS))
-    e4m3 = kind == _lib.E4M3
-    if dtype is None:
-        dtype = torch.bfloat16 if e4m3 else x.dtype
-    yt = _TYPES.get(dtype, -1)
-    if yt not in (_lib.F32, _lib.F16, _lib.BF16):
-        _fail(f"{op}: the output cannot be {dtype}")
-    bp, bt = _vector(op, "bias", bias, R, (torch.float32, dtype, x.dtype))
-    xs, _ = _vector(op, "x_scale", x_scale, M, _F32)
-    ws, _ = _vector(op, "w_scale", w_scale, R, _F32)
-    shape = (*x.shape[:-1], N)
+    if dtype is None or dtype == xd:
+        dtype = torch.bfloat16 if kind == _lib.E4M3 else xd
+    yt = _type(op, "the output", dtype, _VALUES)
+    bp = bt = xs = ws = rp = ldr = zp = 0
+    z = None
+    if bias is not None:
+        bp, bt = _vector(op, "bias", bias, index, R, dtype, _F32, xd)
+    if x_scale is not None:
+        xs, _ = _vector(op, "x_scale", x_scale, index, M, _F32)
+    if w_scale is not None:
+        ws, _ = _vector(op, "w_scale", w_scale, index, R, _F32)
+    shape = (M, N) if x.dim() == 2 else (*x.shape[:-1], N)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
-        ldy = N
+        out = x.new_empty(shape) if dtype == xd else x.new_empty(shape, dtype=dtype)
+        yp, ldy = out.data_ptr(), N
     else:
-        ldy = _same(op, "out", out, shape, dtype)
-    rp, ldr = 0, 0
+        yp, ldy = _same(op, "out", out, index, shape, dtype)
     if residual is not None:
-        ldr = _same(op, "residual", residual, shape, dtype)
-        rp = residual.data_ptr()
-    z, zp = None, 0
+        rp, ldr = _same(op, "residual", residual, index, shape, dtype)
     if save:
-        z = torch.empty((*x.shape[:-1], R), dtype=x.dtype, device=x.device)
+        z = x.new_empty((*shape[:-1], R))
         zp = z.data_ptr()
-    n = _forward_space(gated, M, N, K, kind) if M else 0
-    space, sp = _space(max(n, 0), x)
+    n = _forward_space(gated, M, N, K, kind)
+    space, sp = _space(n, x)
     lib = _lib.load_ffn()
     if gated:
-        st = _launch(x, lib.bvml_ffn_gated, x.data_ptr(), ldx, w.data_ptr(), ldw, bp, xs, ws, M, N,
-                     K, kind, yt, bt, _ACTS[act], out.data_ptr(), ldy, zp, R, sp, n)
+        _launch(op, index, lib.bvml_ffn_gated, x.data_ptr(), ldx, w.data_ptr(), ldw, bp, xs, ws, M,
+                N, K, kind, yt, bt, code, yp, ldy, zp, R, sp, n)
     else:
-        st = _launch(x, lib.bvml_ffn_linear, x.data_ptr(), ldx, w.data_ptr(), ldw, bp, xs, ws, rp,
-                     ldr, M, N, K, kind, yt, bt, _ACTS[act], out.data_ptr(), ldy, zp, R, sp, n)
-    _raise_status(op, st)
+        _launch(op, index, lib.bvml_ffn_linear, x.data_ptr(), ldx, w.data_ptr(), ldw, bp, xs, ws,
+                rp, ldr, M, N, K, kind, yt, bt, code, yp, ldy, zp, R, sp, n)
     return Product(out, z)
 
 
@@ -277,36 +304,37 @@ def gated(x, w, bias=None, act: str = "silu", *, x_scale=None, w_scale=None, dty
 
 
 def _backward(op: str, is_gated: bool, dy, x, w, z, act, need_x, need_w, need_bias):
-    _check(op, dy, x=x, w=w, z=z)
-    kind = _type(op, "x", x.dtype, _HALVES)
-    dt = _type(op, "dy", dy.dtype, (torch.float32, x.dtype))
-    if w.dtype != x.dtype or w.dim() != 2:
-        _fail(f"{op}: w must be a matrix of x's type")
+    index, xd = _index(op, x), x.dtype
+    kind = _type(op, "x", xd, _HALVES)
+    if dy.dtype != xd and dy.dtype != _F32:
+        _fail(f"{op}: the output's gradient is {dy.dtype}, expected {xd} or float32")
+    if w.dtype != xd or w.dim() != 2 or w.get_device() != index:
+        _fail(f"{op}: w must be a matrix of x's type on its device")
     M, K, ldx = _rows(op, "x", x)
     R, Kw, ldw = _rows(op, "w", w)
     if Kw != K or (is_gated and R % 2):
         _fail(f"{op}: w is {tuple(w.shape)}, x has rows of {K}")
     N = R // 2 if is_gated else R
-    if act not in _ACTS:
+    code = _ACTS.get(act)
+    if code is None:
         _fail(f"{op}: unknown activation {act!r}, expected one of " + ", ".join(_ACTS))
-    lddy = _same(op, "dy", dy, (*x.shape[:-1], N), dy.dtype)
+    lead = x.shape[:-1]
+    yp, lddy = _same(op, "dy", dy, index, (*lead, N), dy.dtype)
     zp, ldz = 0, R
     if z is not None:
-        ldz = _same(op, "z", z, (*x.shape[:-1], R), x.dtype)
-        zp = z.data_ptr()
+        zp, ldz = _same(op, "z", z, index, (*lead, R), xd)
     elif is_gated or act != "none":
         _fail(f"{op}: the pre-activations z are needed (forward with save=True)")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-    dw = torch.empty((R, K), dtype=x.dtype, device=x.device) if need_w else None
-    db = torch.empty(R, dtype=x.dtype, device=x.device) if need_bias else None
+    dx = x.new_empty(x.shape) if need_x else None
+    dw = x.new_empty((R, K)) if need_w else None
+    db = x.new_empty((R,)) if need_bias else None
     n = _backward_space(is_gated, M, N, K)
-    space, sp = _space(max(n, 0), x)
+    space, sp = _space(n, x)
     lib = _lib.load_ffn()
-    fn = lib.bvml_ffn_gated_backward if is_gated else lib.bvml_ffn_linear_backward
-    st = _launch(x, fn, dy.data_ptr(), lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, zp, ldz, M, N,
-                 K, kind, dt, _ACTS[act], 0 if dx is None else dx.data_ptr(), K,
-                 0 if dw is None else dw.data_ptr(), K, 0 if db is None else db.data_ptr(), sp, n)
-    _raise_status(op, st)
+    _launch(op, index, lib.bvml_ffn_gated_backward if is_gated else lib.bvml_ffn_linear_backward,
+            yp, lddy, x.data_ptr(), ldx, w.data_ptr(), ldw, zp, ldz, M, N, K, kind,
+            _TYPES[dy.dtype], code, 0 if dx is None else dx.data_ptr(), K,
+            0 if dw is None else dw.data_ptr(), K, 0 if db is None else db.data_ptr(), sp, n)
     return dx, dw, db
 
 

@@ -191,14 +191,26 @@ def test_rows_of_views():
 
 
 def test_plan_reaches_every_kernel():
-    """The sizes of tests/test_gpu_ffn.py name every tile, copy and split."""
+    """The sizes of tests/test_gpu_ffn.py name every tile, copy and split of
+    the forward products and of both gradients together."""
     from tests import test_gpu_ffn as t
     seen = set()
     for M, N, K in t.FORWARD:
         for gated in (False, True):
-            tile, dma, splits = _lib.ffn_plan(M, N * (1 + gated), K, _lib.BF16, 0, gated, K % 8 == 0)
-            seen.add((0, tile, dma, splits > 1))
-    want = {(0, 0, True, False), (0, 0, False, False)}
-    want |= {(0, 256, True, False), (0, 128, True, False), (0, 64, True, False),
-             (0, 64, True, True), (0, 128, False, False)}
+            aligned = K % 8 == 0
+            tile, deep, _, splits = _lib.ffn_plan(M, N * (1 + gated), K, _lib.BF16, 0, gated, aligned)
+            seen.add((tile, deep, aligned, splits > 1))
+    want = {(0, False, a, False) for a in (True, False)}
+    want |= {(256, False, True, False), (128, False, True, False), (128, True, True, False),
+             (64, False, True, False), (64, False, True, True), (128, False, False, False),
+             (128, False, False, True)}
+    assert want <= seen, want - seen
+    seen = set()
+    for M, N, K in t.GRADIENTS:
+        for R in (N, 2 * N):
+            tile, deep, whole, splits = _lib.ffn_plan(M, R, K, _lib.BF16, 3)
+            if K % 8 == 0:
+                seen.add((tile, deep, splits > 1))
+    want = {(256, False, False), (256, False, True), (128, False, False), (128, False, True),
+            (128, True, False), (64, False, False), (64, False, True)}
     assert want <= seen, want - seen
