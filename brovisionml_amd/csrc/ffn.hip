@@ -220,7 +220,8 @@ int backward(const std::string& op, bool gated, const void* dy, long long lddy, 
     sc.dz = own_dz && (dx || dw) ? at : nullptr;
     sc.db = db;
     sc.workspace = reinterpret_cast<float*>(at + space.dz);
-    if (sc.dz || sc.db) BVML_FFN_TRY(launched(op, launch_slope(sc, s)));
+    ColumnSum sums{};
+    if (sc.dz || sc.db) BVML_FFN_TRY(launched(op, launch_slope(sc, &sums, s)));
 
     ProductCall c{};
     c.p = own_dz ? at : dy;
@@ -248,7 +249,8 @@ int backward(const std::string& op, bool gated, const void* dy, long long lddy, 
     weight.layout = kWeightGrad;
     weight.e = plain(dw, lddw, R);
     void* const parts = at + space.dz + space.sums;
-    if (dx && dw) return launched(op, launch_gradients(input, weight, parts, s));
+    if (dx && dw) return launched(op, launch_gradients(input, weight, sums, parts, s));
+    if (db) BVML_FFN_TRY(launched(op, launch_column_sum(sums, s)));
     if (dx && M > 0) return launched(op, launch_product(input, parts, s));
     if (dw) return launched(op, launch_product(weight, parts, s));
     return BVML_FFN_OK;

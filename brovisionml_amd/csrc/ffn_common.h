@@ -105,10 +105,11 @@ __device__ __forceinline__ void store_row(void* base, int type, long long at, in
 // ---------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-__device__ __forceinline__ float sigmoid_fast(float x) {
-    return __builtin_amdgcn_rcpf(1.0f + exp_fast(-x));
+// 1 / (1 + 2^t)
+__device__ __forceinline__ float logistic2(float t) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
+__device__ __forceinline__ float sigmoid_fast(float x) { return logistic2(-kLog2e * x); }
 
 // The normal distribution's Phi(x), with e = exp(-x^2 / 2): erfc by
 // Abramowitz and Stegun's formula 7.1.26, whose error is at most 1.5e-7, on
@@ -122,16 +123,22 @@ __device__ __forceinline__ float normal_cdf(float x, float e) {
     const float tail = 0.5f * p * e;
     return x < 0.0f ? tail : 1.0f - tail;
 }
+__device__ __forceinline__ float normal_bell(float x) {  // exp(-x^2 / 2)
+    return __builtin_amdgcn_exp2f((-0.5f * kLog2e) * x * x);
+}
 
-// 0.5 (1 + tanh(a)) = sigmoid(2 a), a = sqrt(2 / pi) (x + 0.044715 x^3)
+// 0.5 (1 + tanh(a)) = 1 / (1 + exp(-2 a)), a = sqrt(2 / pi) (x + 0.044715 x^3)
 constexpr float kTanhA = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kTanhB = 0.044715f;
+__device__ __forceinline__ float tanh_gate(float x, float x2) {
+    return logistic2(x * __builtin_fmaf(x2, -kLog2e * kTanhA * kTanhB, -kLog2e * kTanhA));
+}
 
 __device__ __forceinline__ float act1(int act, float x) {
     switch (act) {
         case BVML_FFN_RELU: return x < 0.0f ? 0.0f : x;
-        case BVML_FFN_GELU: return x * normal_cdf(x, exp_fast(-0.5f * x * x));
-        case BVML_FFN_GELU_TANH: return x * sigmoid_fast(kTanhA * (x + kTanhB * x * x * x));
+        case BVML_FFN_GELU: return x * normal_cdf(x, normal_bell(x));
+        case BVML_FFN_GELU_TANH: return x * tanh_gate(x, x * x);
         case BVML_FFN_SILU: return x * sigmoid_fast(x);
         default: return x;
     }
@@ -145,22 +152,23 @@ __device__ __forceinline__ void act_slope1(int act, float x, float& value, float
             slope = x > 0.0f ? 1.0f : 0.0f;
             return;
         case BVML_FFN_GELU: {
-            const float e = exp_fast(-0.5f * x * x);
+            const float e = normal_bell(x);
             const float c = normal_cdf(x, e);
             value = x * c;
-            slope = c + x * e * 0.3989422804014327f;
+            slope = __builtin_fmaf(x * e, 0.3989422804014327f, c);
             return;
         }
         case BVML_FFN_GELU_TANH: {
-            const float s = sigmoid_fast(kTanhA * (x + kTanhB * x * x * x));
+            const float x2 = x * x, s = tanh_gate(x, x2);
             value = x * s;
-            slope = s + x * s * (1.0f - s) * kTanhA * (1.0f + 3.0f * kTanhB * x * x);
+            slope = __builtin_fmaf(value * (1.0f - s),
+                                   __builtin_fmaf(x2, 3.0f * kTanhA * kTanhB, kTanhA), s);
             return;
         }
         case BVML_FFN_SILU: {
             const float s = sigmoid_fast(x);
             value = x * s;
-            slope = s + x * s * (1.0f - s);
+            slope = __builtin_fmaf(value, 1.0f - s, s);
             return;
         }
         default:
@@ -169,20 +177,36 @@ __device__ __forceinline__ void act_slope1(int act, float x, float& value, float
     }
 }
 
-// `act` is the same for the whole launch: one scalar branch per vector
+// `act` is the same for the whole launch: one scalar branch per vector.
+#define BVML_FFN_ACTS(CASE) \
+    CASE(BVML_FFN_RELU) CASE(BVML_FFN_GELU) CASE(BVML_FFN_GELU_TANH) CASE(BVML_FFN_SILU)
+
 template <int V>
 __device__ __forceinline__ void activate(int act, float (&v)[V]) {
     switch (act) {
-#define BVML_FFN_CASE(A)                                    \
-    case A:                                                 \
+#define BVML_FFN_CASE(A)                                                    \
+    case A:                                                                 \
         _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = act1(A, v[i]); \
         break;
-        BVML_FFN_CASE(BVML_FFN_RELU)
-        BVML_FFN_CASE(BVML_FFN_GELU)
-        BVML_FFN_CASE(BVML_FFN_GELU_TANH)
-        BVML_FFN_CASE(BVML_FFN_SILU)
+        BVML_FFN_ACTS(BVML_FFN_CASE)
 #undef BVML_FFN_CASE
         default: break;
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void act_slope(int act, const float (&x)[V], float (&value)[V],
+                                          float (&slope)[V]) {
+    switch (act) {
+#define BVML_FFN_CASE(A)                                                                       \
+    case A:                                                                                    \
+        _Pragma("unroll") for (int i = 0; i < V; ++i) act_slope1(A, x[i], value[i], slope[i]); \
+        break;
+        BVML_FFN_ACTS(BVML_FFN_CASE)
+#undef BVML_FFN_CASE
+        default:
+#pragma unroll
+            for (int i = 0; i < V; ++i) act_slope1(BVML_FFN_NONE, x[i], value[i], slope[i]);
     }
 }
 

@@ -41,6 +41,14 @@ bool dma_fits(const ProductCall& c);
 long long product_workspace(int M, int R, int K, int in_type, int layout, bool gated);
 hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s);
 
+// out[c] = the sum of `parts` rows of `cols` floats, of `type` (out null: none).
+struct ColumnSum {
+    const float* part;
+    int parts, cols;
+    void* out;
+    int type;
+};
+
 // Both gradients of one product from the same dz: x's (c.p = dz, c.q = W) and W's
 // (c.p = dz, c.q = x), in one launch where their operands go straight to LDS.
 struct GradientsPlan {
@@ -51,8 +59,9 @@ struct GradientsPlan {
 };
 GradientsPlan plan_gradients(int M, int R, int K);
 long long gradients_workspace(int M, int R, int K);
-hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight, void* workspace,
-                            hipStream_t s);
+// `sums` goes along with them
+hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight,
+                            const ColumnSum& sums, void* workspace, hipStream_t s);
 
 // One translation unit an element type (ffn_product_*.hip).
 struct Product;
@@ -111,10 +120,9 @@ struct SlopeCall {
     void* db;    // null: only dz
     float* workspace;
 };
-// out[c] = the sum of `parts` rows of cols floats
-hipError_t launch_column_sum(const float* part, int parts, int cols, void* out, int type,
-                             hipStream_t s);
+hipError_t launch_column_sum(const ColumnSum& c, hipStream_t s);
 long long slope_workspace(int rows, int R);
-hipError_t launch_slope(const SlopeCall& c, hipStream_t s);
+// (*sums: what is left to do for db)
+hipError_t launch_slope(const SlopeCall& c, ColumnSum* sums, hipStream_t s);
 
 }  // namespace bvml_ffn

@@ -253,7 +253,7 @@ hipError_t launch_norm_grad(const NormGradCall& c, hipStream_t s) {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    return c.dweight ? launch_column_sum(c.workspace, blocks, cols, c.dweight, c.w_type, s)
+    return c.dweight ? launch_column_sum({c.workspace, blocks, cols, c.dweight, c.w_type}, s)
                      : hipSuccess;
 }
 

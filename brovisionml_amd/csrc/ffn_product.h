@@ -37,7 +37,7 @@
 
 #include <type_traits>
 
-#include "ffn_common.h"
+#include "ffn_sums.h"
 
 namespace bvml_ffn {
 
@@ -593,9 +593,11 @@ __global__ __launch_bounds__(256, kWavesPerSimd<BM>) void product_kernel(Product
 // that the other's leave idle.  The product whose workgroups take longer goes
 // first, for a long one started last would keep the launch waiting; before it
 // the parts of the other's last tiles, where only those are split.
+// Last come the workgroups that sum the bias's gradient.
 struct Gradients {
     Product input, weight;
     bool weight_first;
+    ColumnSum sums;
 };
 
 __device__ __forceinline__ int rest_of(const Product& a) {
@@ -609,7 +611,12 @@ __global__ __launch_bounds__(256, kWavesPerSimd<BM>) void gradients_kernel(Gradi
     const Product& second = g.weight_first ? g.input : g.weight;
     const int parts = second.whole > 0 ? rest_of(second) : 0;
     const int longer = first.whole + rest_of(first);
+    const int tiles = longer + second.whole + rest_of(second);
     int b = blockIdx.x;
+    if (b >= tiles) {
+        column_sum<8>(g.sums, b - tiles, reinterpret_cast<float(*)[32]>(lds));
+        return;
+    }
     bool weight = !g.weight_first;
     if (b < parts) {
         b += second.whole;

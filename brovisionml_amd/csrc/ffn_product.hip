@@ -597,17 +597,15 @@ long long gradients_workspace(int M, int R, int K) {
            part_bytes(ceil_div(R, c.bm) * cols, p.weight_whole, p.weight_splits, p.tile);
 }
 
-hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight, void* workspace,
-                            hipStream_t s) {
+hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight,
+                            const ColumnSum& sums, void* workspace, hipStream_t s) {
     if (input.M == 0 || !dma_fits(input) || !dma_fits(weight)) {
-        if (input.M > 0) {
-            const hipError_t e = launch_product(input, workspace, s);
-            if (e != hipSuccess) return e;
-        }
-        return launch_product(weight, workspace, s);
+        hipError_t e = sums.out ? launch_column_sum(sums, s) : hipSuccess;
+        if (e == hipSuccess && input.M > 0) e = launch_product(input, workspace, s);
+        return e == hipSuccess ? launch_product(weight, workspace, s) : e;
     }
     const GradientsPlan p = plan_gradients(input.M, input.K, input.R);
-    Gradients g{product_of(input), product_of(weight), p.weight_first};
+    Gradients g{product_of(input), product_of(weight), p.weight_first, sums};
     lay_out(g.input, input, p.tile, p.input_whole, p.input_splits, workspace);
     const long long ti = (long long)g.input.tiles_m * g.input.tiles_n;
     lay_out(g.weight, weight, p.tile, p.weight_whole, p.weight_splits,

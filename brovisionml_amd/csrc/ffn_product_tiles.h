@@ -33,7 +33,7 @@ hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) 
 
 template <int kIn, int BM, int BN, int S>
 hipError_t launch_both(const Gradients& g, hipStream_t s) {
-    long long groups = 0;
+    long long groups = g.sums.out ? (g.sums.cols + 31) / 32 : 0;
     for (const Product* a : {&g.input, &g.weight})
         groups += a->whole + ((long long)a->tiles_m * a->tiles_n - a->whole) * a->splits;
     if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;

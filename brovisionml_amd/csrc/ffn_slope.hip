@@ -8,6 +8,7 @@
 // inputs give equal bits.
 
 #include "ffn_kernels.h"
+#include "ffn_sums.h"
 
 namespace bvml_ffn {
 
@@ -17,8 +18,9 @@ constexpr int kVec = 8;        // columns a thread
 constexpr int kLanes = 32;     // threads along the columns
 constexpr int kRows = 8;       // threads along the rows
 constexpr int kMostParts = 256;
+constexpr int kSumRuns = 32;
 
-template <bool kGated>
+template <bool kGated, int kAhead>
 __global__ __launch_bounds__(256) void slope_kernel(SlopeCall c, int rows_each) {
     constexpr int kHalves = kGated ? 2 : 1;
     __shared__ float sums[kRows][kHalves][kLanes * kVec];
@@ -33,41 +35,59 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeCall c, int rows_each) 
 #pragma unroll
         for (int i = 0; i < kVec; ++i) s[h][i] = 0.0f;
     if (left > 0) {
-        for (int r = r0 + y; r < r1; r += kRows) {
-            float dy[kVec], z[kVec], d[kVec];
-            load_row<kVec>(c.dy, c.dy_type, (long long)r * c.lddy + n, left, dy);
-            if constexpr (kGated) {
-                float up[kVec], du[kVec];
-                load_row<kVec>(c.z, c.type, (long long)r * c.ldz + n, left, z);
-                load_row<kVec>(c.z, c.type, (long long)r * c.ldz + c.N + n, left, up);
+        // kAhead rows at a time, so that their loads are in flight together
+        for (int r = r0 + y; r < r1; r += kRows * kAhead) {
+            float dy[kAhead][kVec], z[kAhead][kVec], up[kGated ? kAhead : 1][kVec];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    float value, slope;
-                    act_slope1(c.act, z[i], value, slope);
-                    d[i] = dy[i] * up[i] * slope;
-                    du[i] = dy[i] * value;
-                    s[0][i] += d[i];
-                    s[1][i] += du[i];
-                }
-                if (c.dz) {
-                    store_row<kVec>(c.dz, c.type, (long long)r * c.ldd + n, left, d);
-                    store_row<kVec>(c.dz, c.type, (long long)r * c.ldd + c.N + n, left, du);
-                }
-            } else {
-                if (c.z) load_row<kVec>(c.z, c.type, (long long)r * c.ldz + n, left, z);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    float value, slope = 1.0f;
-                    if (c.z) act_slope1(c.act, z[i], value, slope);
-                    d[i] = dy[i] * slope;
-                    s[0][i] += d[i];
-                }
-                if (c.dz) store_row<kVec>(c.dz, c.type, (long long)r * c.ldd + n, left, d);
+            for (int t = 0; t < kAhead; ++t) {
+                const long long at = kAhead == 1 || r + t * kRows < r1 ? r + t * kRows : r;
+                load_row<kVec>(c.dy, c.dy_type, at * c.lddy + n, left, dy[t]);
+                if (kGated || c.z) load_row<kVec>(c.z, c.type, at * c.ldz + n, left, z[t]);
+                if constexpr (kGated) load_row<kVec>(c.z, c.type, at * c.ldz + c.N + n, left, up[t]);
             }
-            // the zeros between the last column and the row's end
-            if (c.dz && left <= kVec)
-                for (int i = R; i < c.ldd; ++i)
-                    static_cast<uint16_t*>(c.dz)[(long long)r * c.ldd + i] = 0;
+#pragma unroll
+            for (int t = 0; t < kAhead; ++t) {
+                const long long at = r + t * kRows;
+                if (kAhead > 1 && at >= r1) break;
+                float d[kVec], du[kVec];
+                // (the activations of the whole vector at once take fewer
+                // branches but more registers, which the gated form has none
+                // left of at 8 waves a SIMD: 16,389 x 8,192 119 us, 128 with
+                // it; 4,805 x 5,120 ungated 34 without, 31 with it)
+                if constexpr (kGated && kAhead == 1) {
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        float value, slope;
+                        act_slope1(c.act, z[t][i], value, slope);
+                        d[i] = dy[t][i] * up[t][i] * slope;
+                        du[i] = dy[t][i] * value;
+                    }
+                } else {
+                    float value[kVec], slope[kVec];
+                    if (kGated || c.z) act_slope<kVec>(c.act, z[t], value, slope);
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        d[i] = dy[t][i];
+                        if (kGated || c.z) d[i] *= slope[i];
+                        if constexpr (kGated) {
+                            d[i] *= up[t][i];
+                            du[i] = dy[t][i] * value[i];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    s[0][i] += d[i];
+                    if constexpr (kGated) s[1][i] += du[i];
+                }
+                if (!c.dz) continue;
+                store_row<kVec>(c.dz, c.type, at * c.ldd + n, left, d);
+                if constexpr (kGated) store_row<kVec>(c.dz, c.type, at * c.ldd + c.N + n, left, du);
+                // the zeros between the last column and the row's end
+                if (left <= kVec)
+                    for (int i = R; i < c.ldd; ++i)
+                        static_cast<uint16_t*>(c.dz)[at * c.ldd + i] = 0;
+            }
         }
     }
     if (!c.db) return;
@@ -87,51 +107,22 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeCall c, int rows_each) 
     }
 }
 
-// out[c] = sum over the parts: 32 interleaved runs of them, then the runs.
-// Bound by latency: a thread has eight of its loads in flight (1,024 rows of
-// 1,024 columns: 39 us with one at a time by 8 runs).
-constexpr int kRuns = 32, kInFlight = 8;
-__global__ __launch_bounds__(32 * kRuns) void column_sum_kernel(const float* part, int parts,
-                                                                int cols, void* out, int type) {
-    __shared__ float sums[kRuns][32];
-    const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-    const int col = blockIdx.x * 32 + x;
-    float t = 0.0f;
-    if (col < cols) {
-        const float* p = part + col;
-        int r = y;
-        for (; r + (kInFlight - 1) * kRuns < parts; r += kInFlight * kRuns) {
-            float v[kInFlight];
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) v[i] = p[(long long)(r + i * kRuns) * cols];
-#pragma unroll
-            for (int i = 0; i < kInFlight; ++i) t += v[i];
-        }
-        for (; r < parts; r += kRuns) t += p[(long long)r * cols];
-    }
-    sums[y][x] = t;
-    __syncthreads();
-    if (y != 0 || col >= cols) return;
-#pragma unroll
-    for (int j = 1; j < kRuns; ++j) t += sums[j][x];
-    if (type == kF32)
-        static_cast<float*>(out)[col] = t;
-    else
-        static_cast<uint16_t*>(out)[col] = to16(t, type);
+__global__ __launch_bounds__(32 * kSumRuns) void column_sum_kernel(ColumnSum c) {
+    __shared__ float sums[kSumRuns][32];
+    column_sum<kSumRuns>(c, blockIdx.x, sums);
 }
 
 int rows_each_of(int rows) {
     const int each = (rows + kMostParts - 1) / kMostParts;
     const int whole = (each + kRows - 1) / kRows * kRows;
-    return whole < 32 ? 32 : whole;
+    return whole < 16 ? 16 : whole;
 }
 
 }  // namespace
 
-hipError_t launch_column_sum(const float* part, int parts, int cols, void* out, int type,
-                             hipStream_t s) {
-    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(32 * kRuns), 0, s, part,
-                       parts, cols, out, type);
+hipError_t launch_column_sum(const ColumnSum& c, hipStream_t s) {
+    hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((c.cols + 31) / 32)), dim3(32 * kSumRuns),
+                       0, s, c);
     return hipGetLastError();
 }
 
@@ -140,19 +131,26 @@ long long slope_workspace(int rows, int R) {
     return (long long)((rows + each - 1) / each) * R * 4;
 }
 
-hipError_t launch_slope(const SlopeCall& c, hipStream_t s) {
+hipError_t launch_slope(const SlopeCall& c, ColumnSum* sums, hipStream_t s) {
     const int each = rows_each_of(c.rows), parts = (c.rows + each - 1) / each;
     const int R = c.gated ? 2 * c.N : c.N;
-    if (parts > 0) {
-        const dim3 grid((unsigned)((c.N + kLanes * kVec - 1) / (kLanes * kVec)), (unsigned)parts);
-        if (c.gated)
-            hipLaunchKernelGGL(slope_kernel<true>, grid, dim3(256), 0, s, c, each);
-        else
-            hipLaunchKernelGGL(slope_kernel<false>, grid, dim3(256), 0, s, c, each);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+    *sums = {c.workspace, parts, R, c.db, c.type};
+    if (parts == 0) return hipSuccess;
+    const dim3 grid((unsigned)((c.N + kLanes * kVec - 1) / (kLanes * kVec)), (unsigned)parts);
+    // two rows at a time where the workgroups do not fill the card: 1,205 x
+    // 5,460 gated 15 to 12 us, but 16,389 x 8,192 120 to 135
+    const bool few = (long long)grid.x * grid.y < 1024;
+#define BVML_FFN_SLOPE(G, A) \
+    hipLaunchKernelGGL((slope_kernel<G, A>), grid, dim3(256), 0, s, c, each)
+    if (c.gated) {
+        if (few) BVML_FFN_SLOPE(true, 2);
+        else BVML_FFN_SLOPE(true, 1);
+    } else {
+        if (few) BVML_FFN_SLOPE(false, 2);
+        else BVML_FFN_SLOPE(false, 1);
     }
-    return c.db ? launch_column_sum(c.workspace, parts, R, c.db, c.type, s) : hipSuccess;
+#undef BVML_FFN_SLOPE
+    return hipGetLastError();
 }
 
 }  // namespace bvml_ffn
