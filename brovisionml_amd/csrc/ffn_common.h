@@ -241,9 +241,12 @@ struct Column {
         if (e.bias) load_row<V>(e.bias, e.bias_type, col, c, bias);
         if (e.w_scale) load_row<V>(e.w_scale, kF32, col, c, scale);
     }
+    // kScaled false: 16-bit operands, which have no scales
+    template <bool kScaled>
     __device__ __forceinline__ void apply(float row_scale, float (&v)[V]) const {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = v[i] * (row_scale * scale[i]) + bias[i];
+        for (int i = 0; i < V; ++i)
+            v[i] = kScaled ? __builtin_fmaf(v[i], row_scale * scale[i], bias[i]) : v[i] + bias[i];
     }
 };
 
@@ -253,7 +256,7 @@ struct Column {
 template <int V>
 __device__ __forceinline__ void finish(const Epilogue& e, const Column<V>& k, int type16, int m,
                                        int n, int c, float (&v)[V], const float (&r)[V]) {
-    k.apply(e.x_scale ? e.x_scale[m] : 1.0f, v);
+    k.template apply<true>(e.x_scale ? e.x_scale[m] : 1.0f, v);
     if (e.z) store_row<V>(e.z, type16, (long long)m * e.ldz + n, c, v);
     activate<V>(e.act, v);
     if (e.residual) {
@@ -269,8 +272,8 @@ __device__ __forceinline__ void finish_gated(const Epilogue& e, const Column<V>&
                                              const Column<V>& ku, int type16, int m, int n, int c,
                                              float (&g)[V], float (&u)[V]) {
     const float s = e.x_scale ? e.x_scale[m] : 1.0f;
-    kg.apply(s, g);
-    ku.apply(s, u);
+    kg.template apply<true>(s, g);
+    ku.template apply<true>(s, u);
     if (e.z) {
         store_row<V>(e.z, type16, (long long)m * e.ldz + n, c, g);
         store_row<V>(e.z, type16, (long long)m * e.ldz + e.N + n, c, u);

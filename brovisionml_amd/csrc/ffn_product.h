@@ -135,6 +135,7 @@ template <int kIn, int kRows, int kWaves, bool kT, bool kRemap, bool kDma>
 struct Copy {
     static constexpr int kSize = kIn == kE4M3 ? 1 : 2;
     static constexpr int kPiece = 16 / kSize;  // elements of 16 bytes
+    static constexpr int kStep = 128 / kSize;  // k of one step
     static constexpr int kParts = kRows / 8 / kWaves;
     static constexpr int kChunks = kRows / 8;  // pieces of a transposed row
     static_assert(kRows % (8 * kWaves) == 0 && kWaves % 4 == 0, "whole copies; one key a lane");
@@ -146,6 +147,7 @@ struct Copy {
     v4i rsrc;
     const char* base;
     int left;
+    long long have;  // transposed: bytes to the end
 
     static __device__ __forceinline__ int across_k(int t, int w, int lane) {
         return ((t * kWaves + w) * 64 + lane) / kChunks;
@@ -175,18 +177,26 @@ struct Copy {
         }
     }
 
-    // The step whose first k is at `from`, `remain` k before the end (none:
-    // zeros, without touching memory).
+    // The first step: its first k is at `from`, `remain` k before the end.
     __device__ __forceinline__ void aim(const char* from, long long ld, int remain) {
         base = from;
         left = remain;
+        have = kT ? remain * ld : 0;
+        describe();
+    }
+    // The one after it (past the end: zeros, without touching memory).
+    __device__ __forceinline__ void next(long long ld) {
+        base += kT ? kStep * ld : 128;
+        left -= kStep;
+        if constexpr (kT) have -= kStep * ld;
+        describe();
+    }
+    __device__ __forceinline__ void describe() {
         if constexpr (kDma) {
             uint32_t bytes = kBufferEnd;
-            if constexpr (kT) {
-                const long long have = (long long)remain * ld;
-                bytes = have < (long long)kBufferEnd ? (uint32_t)have : kBufferEnd;
-            }
-            const uint64_t at = reinterpret_cast<uint64_t>(from);
+            if constexpr (kT)
+                bytes = have < 0 ? 0u : have < (long long)kBufferEnd ? (uint32_t)have : kBufferEnd;
+            const uint64_t at = reinterpret_cast<uint64_t>(base);
             rsrc = (v4i){(int)(uint32_t)at, (int)(uint32_t)(at >> 32) & 0xffff, (int)bytes,
                          kBufferWord3};
         }
@@ -291,12 +301,17 @@ __device__ __forceinline__ void product_tile(const Product& a, const int b, char
     const char* pb = kPT ? a.p + (long long)m0 * 2 : a.p + (long long)m0 * a.ldp;
     const char* qb = kQT ? a.q + (long long)n0 * 2 : a.q + (long long)n0 * a.ldq;
 
-    auto aim = [&](int step) {  // (a step beyond the last: nothing remains)
-        const int k = step * kStep, remain = step < step1 ? a.K - k : 0;
+    {
+        const int k = step0 * kStep, end = step1 < a.steps ? step1 * kStep : a.K;
         const long long at = kQT ? k * a.ldq : (long long)k * kSize;
-        cp.aim(pb + (kPT ? k * a.ldp : (long long)k * kSize), a.ldp, remain);
-        cq.aim(qb + at, a.ldq, remain);
-        if constexpr (kGated) cu.aim(qb + (long long)(a.R / 2) * a.ldq + at, a.ldq, remain);
+        cp.aim(pb + (kPT ? k * a.ldp : (long long)k * kSize), a.ldp, end - k);
+        cq.aim(qb + at, a.ldq, end - k);
+        if constexpr (kGated) cu.aim(qb + (long long)(a.R / 2) * a.ldq + at, a.ldq, end - k);
+    }
+    auto next_step = [&]() {
+        cp.next(a.ldp);
+        cq.next(a.ldq);
+        if constexpr (kGated) cu.next(a.ldq);
     };
     auto start = [&](int t, char* slot) {  // part t of PP + QP
         if (t < PP)
@@ -306,8 +321,7 @@ __device__ __forceinline__ void product_tile(const Product& a, const int b, char
         else
             cu.start(t - PP, rows_q, w, lane, slot + kPBytes);
     };
-    auto start_all = [&](int step, char* slot) {
-        aim(step);
+    auto start_all = [&](char* slot) {
 #pragma unroll
         for (int t = 0; t < PP + QP; ++t) start(t, slot);
     };
@@ -410,12 +424,16 @@ __device__ __forceinline__ void product_tile(const Product& a, const int b, char
 
     if (step0 < step1) {
         // (past the last step a copy is zeros: every step counts the same)
-        start_all(step0, lds);
+        start_all(lds);
         commit(lds);
 #pragma unroll
-        for (int i = 1; i < kSlots - 1; ++i) start_all(step0 + i, lds + i * kSlot);
+        for (int i = 1; i < kSlots - 1; ++i) {
+            next_step();
+            start_all(lds + i * kSlot);
+        }
         arrive();
-        start_all(step0 + kSlots - 1, lds + (kSlots - 1) * kSlot);
+        next_step();
+        start_all(lds + (kSlots - 1) * kSlot);
 #pragma unroll
         for (int r = 0; r < kReads; ++r) read(lds, 0, r, p[0], q[0]);
         int cur = 0;
@@ -423,10 +441,11 @@ __device__ __forceinline__ void product_tile(const Product& a, const int b, char
             const int next = cur == (kSlots - 1) * kSlot ? 0 : cur + kSlot;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                if (kk == 1) {
+                if (kk == 0) {
+                    next_step();  // which the second half starts to copy
+                } else {
                     commit(lds + next);
                     arrive();
-                    aim(s + kSlots);
                 }
                 const char* const from = lds + (kk == 0 ? cur : next);
 #pragma unroll
@@ -547,9 +566,10 @@ __device__ __forceinline__ void product_tile(const Product& a, const int b, char
 #pragma unroll
                 for (int t = 0; t < kTimes; ++t) {
                     const int m = first + t * kGap;
-                    const float s = e.x_scale ? e.x_scale[m < a.M ? m : a.M - 1] : 1.0f;
-                    kv.apply(s, v[t]);
-                    if constexpr (kGated) ku.apply(s, u[t]);
+                    constexpr bool kScaled = kIn == kE4M3;
+                    const float s = kScaled ? e.x_scale[m < a.M ? m : a.M - 1] : 1.0f;
+                    kv.template apply<kScaled>(s, v[t]);
+                    if constexpr (kGated) ku.template apply<kScaled>(s, u[t]);
                 }
                 if (e.z) {
                     store(e.z, type16, e.ldz, n, v);
