@@ -48,7 +48,7 @@ template <int kIn, int kBlocks, int kWaves, bool kGated, bool kWhole>
 __global__ __launch_bounds__(64 * kWaves) void rows_kernel(Product a) {
     constexpr int kHalves = kGated ? 2 : 1;
     constexpr int kSize = kIn == kE4M3 ? 1 : 2, kPiece = 16 / kSize, kStep = 128 / kSize;
-    constexpr int kAhead = kBlocks == 4 ? 1 : kBlocks == 2 ? 2 : kGated ? 2 : 5;
+    constexpr int kAhead = kBlocks > 1 || kGated ? 2 : 5;
     __shared__ v4f sums[kWaves][kHalves][kBlocks][64];
 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -330,13 +330,16 @@ hipError_t launch_rows_of(const Product& a, bool whole, hipStream_t s) {
     if (a.M == 1) return launch_dot_of<kIn, 1, kGated>(a, whole, s);
     if (a.M == 2) return launch_dot_of<kIn, 2, kGated>(a, whole, s);
     if (a.M <= 4) return launch_dot_of<kIn, 4, kGated>(a, whole, s);
-    // 16 waves where the workgroups are few and k is long enough for them
-    const bool wide = a.e.N <= 16 * 256 && a.steps >= 32;
-    if (a.M <= 16)
-        return wide ? launch_rows_one<kIn, 1, 16, kGated>(a, whole, s)
-                    : launch_rows_one<kIn, 1, 8, kGated>(a, whole, s);
-    if (a.M <= 32) return launch_rows_one<kIn, 2, 8, kGated>(a, whole, s);
-    return launch_rows_one<kIn, 4, 8, kGated>(a, whole, s);
+    if (a.M <= 16) {
+        // 16 waves where the workgroups are few and k is long enough for them
+        // (not for the gated form, whose sums do not fit their registers)
+        if constexpr (!kGated) {
+            if (a.e.N <= 16 * 256 && a.steps >= 32)
+                return launch_rows_one<kIn, 1, 16, kGated>(a, whole, s);
+        }
+        return launch_rows_one<kIn, 1, 8, kGated>(a, whole, s);
+    }
+    return launch_rows_one<kIn, 2, 8, kGated>(a, whole, s);
 }
 
 hipError_t launch_rows(const ProductCall& c, hipStream_t s) {
@@ -380,13 +383,16 @@ constexpr TileCost kCosts[] = {
     {128, 128, 256, 4.0, 0.47, 0.45, 0.12},  // 2048^2 x 5120: 45 us, 59 with two slots
     {64, 128, 512, 3.0, 0.55, 0.33, 0.12},   // 2048 x 1024 x 5120: 30 us
 };
+constexpr int kFewRows = 32;
 // A second launch, and a byte of a part written and read.
 constexpr double kJoin = 5.0, kJoinBytes = 8.0 / 4e6;
 
 }  // namespace
 
 ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
-    if (layout == kForward && M <= 64) return {kTileRows, dma, 0, 1};
+    // (every workgroup of the few-rows kernel reads all of x: 64 rows of 1,280 by
+    // 5,120 columns take it 15 us, the 64 x 128 tiles 10; 32 rows 8)
+    if (layout == kForward && M <= kFewRows) return {kTileRows, dma, 0, 1};
     const int n = gated ? R / 2 : R;
     const long long steps = ceil_div(K, step_of(in_type));
     ProductPlan best{kTile128, dma, 0, 1};

@@ -297,7 +297,7 @@ def _usual(gated: bool, x, w, bias, act, residual):
     return Product(out, None)
 
 
-_FEW = 64  # rows up to which a forward product needs no workspace
+_FEW = 32  # rows up to which a forward product needs no workspace
 
 
 def _forward(op: str, gated: bool, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out):

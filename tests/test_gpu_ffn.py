@@ -58,9 +58,10 @@ def quantised(v):
 # ---------------------------------------------------------------------------
 # linear and gated, forward
 # ---------------------------------------------------------------------------
-# M, N, K: the few-rows kernel with one, two and four blocks of rows; each
-# tile; split sums; sizes around a tile's and a step's edges
-FORWARD = [(1, 1, 1), (1, 1280, 5120), (3, 40, 72), (16, 16, 64), (17, 24, 200), (33, 50, 130),
+# M, N, K: one to four rows, the few-rows kernel with one and two blocks of
+# rows; each tile; split sums; sizes around a tile's and a step's edges
+FORWARD = [(1, 1, 1), (1, 1280, 5120), (3, 40, 72), (16, 16, 64), (16, 700, 2312), (17, 24, 200),
+           (32, 90, 1000), (31, 19, 77), (33, 50, 130),
            (64, 1000, 1024), (65, 64, 64), (100, 136, 96), (129, 130, 1032), (252, 1000, 1024),
            (300, 257, 264), (1000, 1111, 136), (1281, 2056, 520), (2100, 5128, 72),
            (130, 5, 2048), (77, 513, 1), (200, 31, 33), (2000, 2040, 2056), (130, 70, 1033),
