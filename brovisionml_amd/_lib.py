@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 
-from .build import LIB, LIB_FFN, LIB_REFINE
+from .build import LIB, LIB_FFN, LIB_FFN_CALL, LIB_REFINE
 
 # Status codes (include/bvml_dsine.h)
 OK = 0
@@ -258,6 +258,22 @@ def load_ffn(path: str = LIB_FFN) -> ctypes.CDLL:
         getattr(lib, name).restype = ctypes.c_char_p
     _ffn = lib
     return lib
+
+
+def load_ffn_call(path: str = LIB_FFN_CALL):
+    """The extension module of csrc/ffn_call.cpp; raises if it was not built."""
+    import importlib.machinery
+    import importlib.util
+    load_ffn()
+    if not os.path.exists(path):
+        raise RuntimeError(
+            f"brovisionml_amd: native module {path} is missing; run "
+            "`python -m brovisionml_amd.build` first")
+    loader = importlib.machinery.ExtensionFileLoader("_ffn_call", path)
+    module = importlib.util.module_from_spec(
+        importlib.util.spec_from_file_location("_ffn_call", path, loader=loader))
+    loader.exec_module(module)
+    return module
 
 
 def ffn_last_error() -> str:

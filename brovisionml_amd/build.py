@@ -18,6 +18,9 @@
   libbvml_ffn.so          the feed-forward operators (include/bvml_ffn.h): HIP
                           kernels behind a C ABI of their own; extern "C"
                           symbols only
+  _ffn_call.so            the usual call of those operators from Python
+                          (ffn_call.cpp): a CPython extension module over
+                          libbvml_ffn.so
   libbrotensor_subset.so  the brotensor::Tensor subset of
                           include/brotensor/tensor.h, for standalone use and
                           the C++ tests; a brovisionml build links brotensor
@@ -28,6 +31,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -41,6 +45,7 @@ LIB_TENSOR = os.path.join(LIBDIR, "libbrotensor_subset.so")
 LIB_REFINE = os.path.join(LIBDIR, "libbvml_dsine_refine.so")
 LIB_REFINE_CXX = os.path.join(LIBDIR, "libbvml_dsine_refine_cxx.so")
 LIB_FFN = os.path.join(LIBDIR, "libbvml_ffn.so")
+LIB_FFN_CALL = os.path.join(LIBDIR, "_ffn_call.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -92,6 +97,7 @@ REFINE_HIP_SOURCES = [os.path.join(CSRC, "refiner_conv.hip"),
 FFN_SOURCES = [os.path.join(CSRC, name + ".hip") for name in (
     "ffn_product_bf16", "ffn_product_f16", "ffn_product_e4m3", "ffn_product", "ffn_norm",
     "ffn_slope", "ffn")]
+FFN_CALL_SOURCE = os.path.join(CSRC, "ffn_call.cpp")
 # host C++ against the HIP runtime headers
 HIP_HOST_FLAGS = ["-D__HIP_PLATFORM_AMD__", "-isystem", os.path.join(ROCM, "include")]
 
@@ -117,10 +123,14 @@ def _build_ffn(objdir: str, status_obj: str) -> None:
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-o", LIB_FFN + ".tmp", *objs, status_obj,
           "-Wl,--version-script=" + os.path.join(CSRC, "libbvml_ffn.map")])
     _install(LIB_FFN + ".tmp", LIB_FFN)
+    _run([CXX, *CXX_FLAGS, "-I", INCLUDE, "-isystem", sysconfig.get_path("include"), "-shared",
+          "-o", LIB_FFN_CALL + ".tmp", FFN_CALL_SOURCE, "-L", LIBDIR, "-lbvml_ffn",
+          "-Wl,-rpath,$ORIGIN"])
+    _install(LIB_FFN_CALL + ".tmp", LIB_FFN_CALL)
 
 
 def build_library() -> str:
-    """Builds the six libraries; returns the DSINE ops' C ABI library's path."""
+    """Builds the six libraries and the extension module; returns the DSINE ops' C ABI library's path."""
     os.makedirs(LIBDIR, exist_ok=True)
     objdir = os.path.join(PKG, "_build")
     os.makedirs(objdir, exist_ok=True)

@@ -51,8 +51,17 @@ def _fail(msg: str):
     raise RuntimeError(_WHO + msg)
 
 
-# The checks below take the cheapest queries for the usual call: at a few rows
-# the kernels take less time than they do.
+# At a few rows the kernels take less time than a call's checks: the usual call
+# runs in C (csrc/ffn_call.cpp), which returns None for any other, and the
+# checks below take the cheapest queries.
+@lru_cache(maxsize=None)
+def _call():
+    module = _lib.load_ffn_call()
+    module.setup(torch.float16, torch.bfloat16, torch.float32, torch.uint8, _ACTS, _device,
+                 _stream)
+    return module
+
+
 _VALUES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _HALVES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _OPERANDS = {**_HALVES, torch.float8_e4m3fn: _lib.E4M3}
@@ -147,29 +156,6 @@ def _space(n: int, like):
 # ---------------------------------------------------------------------------
 # the norm
 # ---------------------------------------------------------------------------
-def _usual_norm(x, residual, weight, eps):
-    """As _usual: contiguous tensors of one type, residual and weight given."""
-    xd, index = x.dtype, x.get_device()
-    kind = _VALUES.get(xd)
-    if (kind is None or index < 0 or residual is None or weight is None or residual.dtype != xd
-            or weight.dtype != xd or residual.get_device() != index
-            or weight.get_device() != index or x.dim() == 0
-            or not (x.is_contiguous() and residual.is_contiguous() and weight.is_contiguous())
-            or _device() != index):
-        return None
-    shape, cols = x.shape, x.shape[-1]
-    n = x.numel()
-    if residual.shape != shape or weight.numel() != cols or n == 0:
-        return None
-    y, stream = x.new_empty(shape), x.new_empty(shape)
-    status = _lib.load_ffn().bvml_ffn_add_rms_norm(
-        x.data_ptr(), cols, residual.data_ptr(), cols, weight.data_ptr(), n // cols, cols, eps, kind,
-        kind, kind, y.data_ptr(), cols, stream.data_ptr(), cols, 0, 0, _stream(index))
-    if status != _lib.OK:
-        _fail(f"add_rms_norm: {_lib.ffn_last_error()} (status {status})")
-    return Norm(y, None, stream, None)
-
-
 def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, *, dtype=None,
                  save: bool = False) -> Norm:
     """s = x + residual and y = s / sqrt(mean(s^2) + eps) * weight over the last
@@ -178,10 +164,10 @@ def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, *, dtype=None
     y = q * scale), `stream` = s in x's type (x itself without a residual) and,
     with save, the rows' rstd for the backward pass.  The weight is float32
     or of x's type; None means ones."""
-    if dtype is None and not save:
-        norm = _usual_norm(x, residual, weight, eps)
-        if norm is not None:
-            return norm
+    if not save:
+        done = _call().norm(x, residual, weight, eps, dtype)
+        if done is not None:
+            return Norm(done[0], None, done[1], None)
     op = "add_rms_norm"
     index, xd = _index(op, x), x.dtype
     xt = _type(op, "x", xd, _VALUES)
@@ -256,50 +242,6 @@ def _backward_space(gated: bool, M: int, N: int, K: int) -> int:
             else lib.bvml_ffn_linear_backward_workspace)(M, N, K)
 
 
-def _usual(gated: bool, x, w, bias, act, residual):
-    """The usual call, a product of contiguous 16-bit matrices without scales,
-    with every check in the fewest steps: Product, or None where anything is
-    out of the ordinary (the checks of _forward then say what).  2 us less
-    than those, of the 8 us that a product of one row takes."""
-    xd, index = x.dtype, x.get_device()
-    kind, code = _HALVES.get(xd), _ACTS.get(act)
-    if (kind is None or code is None or index < 0 or w.dtype != xd or w.get_device() != index
-            or not (x.is_contiguous() and w.is_contiguous()) or x.dim() != 2 or w.dim() != 2):
-        return None
-    (M, K), (R, Kw) = x.shape, w.shape
-    N = R // 2 if gated else R
-    if Kw != K or M == 0 or N == 0 or K == 0 or (gated and R % 2) or _device() != index:
-        return None
-    bp = bt = rp = 0
-    if bias is not None:
-        if (bias.dtype != xd or bias.get_device() != index or bias.numel() != R
-                or not bias.is_contiguous()):
-            return None
-        bp, bt = bias.data_ptr(), kind
-    out = x.new_empty((M, N))
-    if residual is not None:
-        if (residual.dtype != xd or residual.get_device() != index
-                or residual.shape != out.shape or not residual.is_contiguous()):
-            return None
-        rp = residual.data_ptr()
-    n = 0 if M <= _FEW else _forward_space(gated, M, N, K, kind)
-    space, sp = _space(n, x) if n else (None, 0)
-    if gated:
-        status = _lib.load_ffn().bvml_ffn_gated(
-            x.data_ptr(), K, w.data_ptr(), K, bp, 0, 0, M, N, K, kind, kind, bt, code,
-            out.data_ptr(), N, 0, R, sp, n, _stream(index))
-    else:
-        status = _lib.load_ffn().bvml_ffn_linear(
-            x.data_ptr(), K, w.data_ptr(), K, bp, 0, 0, rp, N, M, N, K, kind, kind, bt, code,
-            out.data_ptr(), N, 0, R, sp, n, _stream(index))
-    if status != _lib.OK:
-        _fail(f"{'gated' if gated else 'linear'}: {_lib.ffn_last_error()} (status {status})")
-    return Product(out, None)
-
-
-_FEW = 32  # rows up to which a forward product needs no workspace
-
-
 def _forward(op: str, gated: bool, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out):
     index, xd = _index(op, x), x.dtype
     kind = _type(op, "x", xd, _OPERANDS)
@@ -363,10 +305,10 @@ def linear(x, w, bias=None, act: str = "none", residual=None, *, x_scale=None, w
     output's (and the residual's), x's type or float32 (from float8: bfloat16
     by default, or float16 or float32).  `out` may be `residual` itself.
     Returns Product(y, z): z the pre-activations in x's type, with save."""
-    if x_scale is None and w_scale is None and dtype is None and not save and out is None:
-        product = _usual(False, x, w, bias, act, residual)
-        if product is not None:
-            return product
+    if x_scale is None and w_scale is None and not save and out is None:
+        y = _call().product(x, w, bias, act, residual, False, dtype)
+        if y is not None:
+            return Product(y, None)
     return _forward("linear", False, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out)
 
 
@@ -375,10 +317,10 @@ def gated(x, w, bias=None, act: str = "silu", *, x_scale=None, w_scale=None, dty
     """h = act(x wg^T + bg) * (x wu^T + bu) for x (..., K) and w = [wg; wu]
     (2N, K), in one kernel; types as linear.  Returns Product(h, z): z (..., 2N)
     the pre-activations of both halves, with save."""
-    if x_scale is None and w_scale is None and dtype is None and not save and out is None:
-        product = _usual(True, x, w, bias, act, None)
-        if product is not None:
-            return product
+    if x_scale is None and w_scale is None and not save and out is None:
+        y = _call().product(x, w, bias, act, None, True, dtype)
+        if y is not None:
+            return Product(y, None)
     return _forward("gated", True, x, w, bias, act, None, x_scale, w_scale, dtype, save, out)
 
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -214,3 +215,27 @@ def test_plan_reaches_every_kernel():
     want = {(256, False, False), (256, False, True), (128, False, False), (128, False, True),
             (128, True, False), (64, False, False), (64, False, True)}
     assert want <= seen, want - seen
+
+
+def test_usual_call_declines_the_rest():
+    """The C form of the usual call returns None, with no error left set and no
+    reference kept, for whatever is not a tensor of its own on a HIP device."""
+    call = ffn._call()
+    x = torch.zeros(4, 4, dtype=torch.bfloat16)
+    odd = (x, x.float(), x[:, ::2], x.to(torch.float8_e4m3fn), torch.zeros(0), torch.zeros(()),
+           torch.zeros([1] * 9), None, 3, "x", object())
+    own = [o for o in odd if o is not None and not isinstance(o, (int, str))]  # shared by others
+    before = [sys.getrefcount(o) for o in own]
+    for a in odd:
+        for b in odd:
+            assert call.product(a, b, None, "none", None, False, None) is None
+            assert call.product(x, a, b, "silu", None, True, torch.bfloat16) is None
+            assert call.norm(a, b, x, 1e-6, None) is None
+            assert call.norm(x, x, a, b, torch.float32) is None
+    assert call.product(x, x, None, [], None, False, None) is None
+    del a, b
+    assert [sys.getrefcount(o) for o in own] == before
+    with pytest.raises(TypeError):
+        call.product(x)
+    with pytest.raises(TypeError):
+        call.norm(x)

@@ -418,3 +418,38 @@ def test_long_rows_apart(cuda):
     for which, got, want in zip(("dx", "dw", "db"), ffn.linear_backward(dy, x, w),
                                 orc.grads(dy, x, w, None, "none", False, BF)):
         within(which, got, *want)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 64), (20, 72, 200), (65, 64, 4096), (300, 130, 96)])
+def test_usual_call_is_the_general_one(M, N, K):
+    """The C form of a usual call gives the general form's bits, where a dtype
+    is named too, and keeps no memory."""
+    torch.manual_seed(M)
+    make = dict(device="cuda", dtype=torch.bfloat16)
+    x, w = torch.randn(M, K, **make), torch.randn(2 * N, K, **make) / 8
+    b, r = torch.randn(2 * N, **make), torch.randn(M, 2 * N, **make)
+    g, call = torch.randn(K, **make), ffn._call()
+
+    def usual(dtype):
+        return (call.product(x, w, b, "gelu", r, False, dtype),
+                call.product(x, w, None, "silu", None, True, dtype),
+                *call.norm(x, x, g, 1e-6, dtype))
+
+    want = (ffn._forward("linear", False, x, w, b, "gelu", r, None, None, None, False, None).y,
+            ffn._forward("gated", True, x, w, None, "silu", None, None, None, None, False, None).y,
+            *(lambda n: (n.y, n.stream))(ffn.add_rms_norm(x, x, g, 1e-6, save=True)))
+    for dtype in (None, torch.bfloat16):
+        for got, ref in zip(usual(dtype), want):
+            assert torch.equal(got, ref)
+    assert call.product(x, w, b, "gelu", r, False, torch.float32) is None
+    assert call.product(x, w, b, "gelu", r[:, :-1], False, None) is None
+    assert call.product(x, w[:-1], None, "silu", None, True, None) is None
+    assert call.product(x, w, b, "sigmoid", None, False, None) is None
+    assert call.norm(x, x, g, 1e-6, torch.float32) is None
+    assert call.norm(x, x, g[:-1], 1e-6, None) is None
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(50):
+        usual(None)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == held
