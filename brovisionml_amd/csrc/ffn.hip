@@ -406,8 +406,9 @@ int bvml_ffn_plan(int M, int R, int K, int in_type, int layout, int gated, int a
         p = {g.tile, true, g.input_splits > 1 ? g.input_whole : g.weight_whole,
              g.input_splits > 1 ? g.input_splits : g.weight_splits};
     }
-    if (tile) *tile = p.tile == kTileRows ? 0 : p.tile == kTile256 ? 256 : p.tile == kTile64 ? 64 : 128;
-    if (deep) *deep = p.tile == kTile128Deep;
+    static const int kRows[] = {256, 128, 128, 64, 64, 0};  // by Tile
+    if (tile) *tile = kRows[p.tile];
+    if (deep) *deep = p.tile == kTile128Deep || p.tile == kTileSquare;
     if (whole) *whole = p.whole;
     if (splits) *splits = p.splits;
     return BVML_FFN_OK;

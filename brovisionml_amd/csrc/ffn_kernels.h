@@ -24,8 +24,9 @@ struct ProductCall {
 };
 
 // 256 x 256; 128 x 128 with two LDS slots (two workgroups a CU) or four (one);
-// 64 x 128 with three (two a CU); the few-rows kernel.
-enum Tile { kTile256 = 0, kTile128 = 1, kTile128Deep = 2, kTile64 = 3, kTileRows = 4 };
+// 64 x 128 with three and 64 x 64 with four (two a CU; the latter not gated); the
+// few-rows kernel.
+enum Tile { kTile256 = 0, kTile128 = 1, kTile128Deep = 2, kTile64 = 3, kTileSquare = 4, kTileRows = 5 };
 
 struct ProductPlan {
     int tile;    // a Tile

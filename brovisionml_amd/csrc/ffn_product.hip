@@ -370,8 +370,8 @@ namespace {
 
 // What a tile costs, in us, measured on bf16 products of 1,280 to 8,192 terms:
 // `fixed` for its first copies and its epilogue, `step` for 128 bytes of k with
-// the card full and `idle` with one workgroup on half of the CUs at most.
-// `room`: workgroups on the card at once.
+// the card full and `idle` with half of that at most.
+// `room`: workgroups on the card at once, one or two a CU.
 // `across`: what an operand read across its rows adds to a step.
 struct TileCost {
     int bm, bn, room;
@@ -381,24 +381,29 @@ constexpr TileCost kCosts[] = {
     {256, 256, 256, 9.0, 1.42, 1.03, 0.06},  // 4096^2 x 8192 at 1350 TFLOP/s
     {128, 128, 512, 5.0, 0.87, 0.65, 0.12},  // 1130
     {128, 128, 256, 4.0, 0.47, 0.45, 0.12},  // 2048^2 x 5120: 45 us, 59 with two slots
-    {64, 128, 512, 3.0, 0.55, 0.33, 0.12},   // 2048 x 1024 x 5120: 30 us
+    {64, 128, 512, 3.0, 0.55, 0.33, 0.12},   // 2048 x 1024 x 5120: 29 us, 34 with 64 x 64
+    {64, 64, 512, 2.8, 0.40, 0.19, 0.09},    // 512 x 1280 x 5120: 18 us, 26 with 64 x 128
 };
+// With part of the card's room taken, 0 to 1.  Up to one workgroup a CU costs
+// `idle`; the first second one makes its CU the last to finish (64 x 64 tiles
+// of 5,120 terms: 256 of them 19 us, 384 33, 512 34).  Where one fills a CU, the
+// step grows with the CUs at work.
+double step_cost(const TileCost& c, double full) {
+    if (full <= 0.5) return c.idle;
+    const double over = 2.0 * full - 1.0;
+    return c.idle + (c.step - c.idle) * (c.room > 256 ? 0.8 + 0.2 * over : over);
+}
 constexpr int kFewRows = 32;
 // A second launch, and a byte of a part written and read.
 constexpr double kJoin = 5.0, kJoinBytes = 8.0 / 4e6;
 
-}  // namespace
-
-ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
-    // (every workgroup of the few-rows kernel reads all of x: 64 rows of 1,280 by
-    // 5,120 columns take it 15 us, the 64 x 128 tiles 10; 32 rows 8)
-    if (layout == kForward && M <= kFewRows) return {kTileRows, dma, 0, 1};
+ProductPlan search_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
     const int n = gated ? R / 2 : R;
     const long long steps = ceil_div(K, step_of(in_type));
     ProductPlan best{kTile128, dma, 0, 1};
     double least = 1e30;
-    for (int tile = kTile256; tile <= kTile64; ++tile) {
-        if (!dma && tile != kTile128) continue;
+    for (int tile = kTile256; tile <= kTileSquare; ++tile) {
+        if ((!dma && tile != kTile128) || (gated && tile == kTileSquare)) continue;
         const TileCost& c = kCosts[tile];
         const long long tiles = ceil_div(M, c.bm) * ceil_div(n, gated ? c.bn / 2 : c.bn);
         // rounds of a full card, then what is left over: one workgroup a tile
@@ -413,8 +418,7 @@ ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gate
             double t = rounds;
             if (left > 0) {
                 const double full = (double)(left * s) / c.room;
-                const double step = full <= 0.5 ? c.idle : c.idle + (c.step - c.idle) * (2 * full - 1);
-                t += c.fixed + each * step * slower;
+                t += c.fixed + each * step_cost(c, full) * slower;
             }
             if (s > 1) t += kJoin + (double)(left * s) * c.bm * c.bn * kJoinBytes;
             if (t < least) {
@@ -424,6 +428,28 @@ ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gate
         }
     }
     return best;
+}
+
+}  // namespace
+
+// (A call asks three times, for its workspace with and without direct copies
+// and for its launch, and a search takes 0.4 us: a thread keeps its last
+// plans, by their sizes.)
+ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
+    // (every workgroup of the few-rows kernel reads all of x: 64 rows of 1,280 by
+    // 5,120 columns take it 15 us, the 64 x 64 tiles 7; 32 rows 8)
+    if (layout == kForward && M <= kFewRows) return {kTileRows, dma, 0, 1};
+    struct Known {
+        int M, R, K, kind;
+        ProductPlan plan;
+    };
+    thread_local Known known[64] = {};
+    const int kind = ((in_type * 4 + layout) * 2 + gated) * 2 + dma;
+    const unsigned h = (unsigned)M * 31u + (unsigned)R * 17u + (unsigned)K + (unsigned)kind;
+    Known& k = known[h % 64u];
+    if (k.M != M || k.R != R || k.K != K || k.kind != kind)
+        k = {M, R, K, kind, search_product(M, R, K, in_type, layout, gated, dma)};
+    return k.plan;
 }
 
 namespace {
@@ -522,7 +548,7 @@ GradientsPlan search_gradients(int M, int R, int K) {
     GradientsPlan best{kTile128, false, 0, 1, 0, 1};
     double least = 1e30;
     const long long si = ceil_div(R, 64), sw = ceil_div(M, 64);  // steps of a tile
-    for (int tile = kTile256; tile <= kTile64; ++tile) {
+    for (int tile = kTile256; tile <= kTileSquare; ++tile) {
         const TileCost& c = kCosts[tile];
         const double bytes = (double)c.bm * c.bn * kJoinBytes;
         const long long cols = ceil_div(K, c.bn);

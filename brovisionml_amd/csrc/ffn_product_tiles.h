@@ -27,7 +27,13 @@ hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) 
         case kTile256: return launch_one<kIn, 256, 256, 2, PT, QT, G, true>(a, s);
         case kTile128: return launch_one<kIn, 128, 128, 2, PT, QT, G, true>(a, s);
         case kTile128Deep: return launch_one<kIn, 128, 128, 4, PT, QT, G, true>(a, s);
-        default: return launch_one<kIn, 64, 128, 3, PT, QT, G, true>(a, s);
+        case kTile64: return launch_one<kIn, 64, 128, 3, PT, QT, G, true>(a, s);
+        default:
+            // (half of 64 columns is no 32 x 32 block for each of two waves)
+            if constexpr (G)
+                return hipErrorInvalidConfiguration;
+            else
+                return launch_one<kIn, 64, 64, 4, PT, QT, G, true>(a, s);
     }
 }
 
@@ -48,7 +54,8 @@ hipError_t launch_gradient_tiles(const Gradients& g, int tile, hipStream_t s) {
         case kTile256: return launch_both<kIn, 256, 256, 2>(g, s);
         case kTile128: return launch_both<kIn, 128, 128, 2>(g, s);
         case kTile128Deep: return launch_both<kIn, 128, 128, 4>(g, s);
-        default: return launch_both<kIn, 64, 128, 3>(g, s);
+        case kTile64: return launch_both<kIn, 64, 128, 3>(g, s);
+        default: return launch_both<kIn, 64, 64, 4>(g, s);
     }
 }
 

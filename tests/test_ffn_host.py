@@ -203,8 +203,8 @@ def test_plan_reaches_every_kernel():
             seen.add((tile, deep, aligned, splits > 1))
     want = {(0, False, a, False) for a in (True, False)}
     want |= {(256, False, True, False), (128, False, True, False), (128, True, True, False),
-             (64, False, True, False), (64, False, True, True), (128, False, False, False),
-             (128, False, False, True)}
+             (64, False, True, False), (64, False, True, True), (64, True, True, False),
+             (64, True, True, True), (128, False, False, False), (128, False, False, True)}
     assert want <= seen, want - seen
     seen = set()
     for M, N, K in t.GRADIENTS:
@@ -213,7 +213,8 @@ def test_plan_reaches_every_kernel():
             if K % 8 == 0:
                 seen.add((tile, deep, splits > 1))
     want = {(256, False, False), (256, False, True), (128, False, False), (128, False, True),
-            (128, True, False), (64, False, False), (64, False, True)}
+            (128, True, False), (64, False, False), (64, False, True), (64, True, False),
+            (64, True, True)}
     assert want <= seen, want - seen
 
 
