@@ -1,10 +1,17 @@
 // RMS norm with the residual's addition, and its gradient.
 //
+//   s = x + residual,  rstd = 1 / sqrt(mean(s^2) + eps),  y = s rstd w
+//   with n = s rstd and a = dy w:  ds = dstream + rstd (a - n mean(a n)),
+//                                  dw = sum over rows of dy n
+//
 // Bound by memory: a row is read once into registers, its sum of squares (and
 // for 8-bit output its largest magnitude) taken across the team of threads
-// that hold it, and every output written from the registers.  A team is a
-// wave up to 2,048 columns (four rows a workgroup, no barrier), a workgroup
-// of 256 or 1,024 threads beyond.
+// that hold it, and every output written from the registers.  Statistics and
+// sums are fp32.  A team is a workgroup of a wave for every 512 columns; rows
+// of one wave share a workgroup of four (BVML_FFN_TEAMS below, with the times).
+//
+// 4805 x 1280 from fp32 to 8 bits, the sum stored too: 14.6 us, 5.5 TB/s.  The
+// gradient of 65541 x 1024: 119 us, 4.5 TB/s, with 5 of them the weight's sums.
 
 #include "ffn_kernels.h"
 
@@ -117,7 +124,8 @@ __global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_kernel(NormCal
 }
 
 // A team walks rows `teams` apart and keeps its columns' part of the weight's
-// gradient in registers; a workgroup leaves one partial row.
+// gradient in registers; a workgroup leaves one partial row, and a second
+// launch sums those in their order: no atomics, equal bits for equal inputs.
 template <int kTeam, int kV>
 __global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_grad_kernel(NormGradCall c) {
     constexpr int kTeams = kTeam == 64 ? 4 : 1;
@@ -201,39 +209,65 @@ __global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_grad_kernel(No
     }
 }
 
+// How a row is dealt out, as (threads of a team, 8-column pieces of each): a
+// wave for every 512 columns, so that a thread has one piece, a row's loads are
+// all on their way at once, and the gradient, which holds four values a
+// column, keeps its waves on the SIMD.  us, bf16, with what else could be:
+//               1 x 1280  norm      192 threads 2.7   a wave, 3 pieces 4.2
+//           16384 x 1280                        30.4                  31.5   256 threads 33.9
+//           16384 x 2048            256         39.8          4       45.2
+//            8192 x 2560            320         29.8  256, 2          31.1
+//            4805 x 1280  gradient  192         21.6  64, 3           24.1
+//            8192 x 2560            320         42.1  256, 2          52.8   512 threads 43.5
+//            4096 x 5120            640         43.6  512, 2          57.3   1024 threads 60.2
+// (and 512, 2 for the norm of 4096 x 5120: 31.9, 640 threads 33.0).  Up to
+// 1,024 columns the norm's teams are of 128 (16384 x 1024: 22.3, a wave's two
+// pieces 23.9; one row 2.6 and 3.3), the gradient's of a wave, four of which
+// leave one partial row (37.4 with its sum, 38.8).
+#define BVML_FFN_TEAMS(GO, UP_TO_1024)           \
+    switch ((cols + 511) / 512) {                \
+        case 0: case 1: GO(64, 1) break;         \
+        case 2: UP_TO_1024 break;                \
+        case 3: GO(192, 1) break;                \
+        case 4: GO(256, 1) break;                \
+        case 5: GO(320, 1) break;                \
+        case 6: GO(384, 1) break;                \
+        case 7: case 8: GO(512, 1) break;        \
+        case 9: case 10: GO(640, 1) break;       \
+        case 11: case 12: GO(768, 1) break;      \
+        case 13: case 14: case 15: case 16:      \
+            GO(1024, 1) break;                   \
+        default:                                 \
+            if (cols <= 16384) { GO(1024, 2) }   \
+            else { GO(1024, 4) }                 \
+    }
+
+// Workgroups of the gradient: as many a CU as stay on it together, found by the
+// step in time beyond them (8192 x 2560: 1,280 workgroups 42 us, 1,536 52; fewer
+// hide less, 768 47), or one where rows are long and partial rows cost more
+// (700 x 32000: 76 us, two 89).
 int grad_blocks(int rows, int cols) {
-    const int teams = cols <= 2048 ? (rows + 3) / 4 : rows;
-    const int most = cols <= 2048 ? 1024 : 512;
+    const int waves = (cols + 511) / 512;
+    const int each = waves <= 2    ? 4
+                     : waves == 3  ? 10
+                     : waves == 4  ? 8
+                     : waves <= 6  ? 5
+                     : waves <= 8  ? 4
+                     : waves <= 16 ? 2
+                                   : 1;
+    const int most = 256 * each;
+    const int teams = waves <= 2 ? (rows + 3) / 4 : rows;
     return teams < most ? teams : most;
 }
 
 }  // namespace
-
-#define BVML_FFN_TEAMS(GO)                      \
-    if (cols <= 512) {                          \
-        GO(64, 1)                               \
-    } else if (cols <= 1024) {                  \
-        GO(64, 2)                               \
-    } else if (cols <= 1536) {                  \
-        GO(64, 3)                               \
-    } else if (cols <= 2048) {                  \
-        GO(64, 4)                               \
-    } else if (cols <= 4096) {                  \
-        GO(256, 2)                              \
-    } else if (cols <= 8192) {                  \
-        GO(256, 4)                              \
-    } else if (cols <= 16384) {                 \
-        GO(1024, 2)                             \
-    } else {                                    \
-        GO(1024, 4)                             \
-    }
 
 hipError_t launch_norm(const NormCall& c, hipStream_t s) {
     const int cols = c.cols;
 #define BVML_FFN_GO(T, V)                                                                   \
     hipLaunchKernelGGL((norm_kernel<T, V>), dim3((unsigned)(T == 64 ? (c.rows + 3) / 4 : c.rows)), \
                        dim3(T == 64 ? 256 : T), 0, s, c);
-    BVML_FFN_TEAMS(BVML_FFN_GO)
+    BVML_FFN_TEAMS(BVML_FFN_GO, BVML_FFN_GO(128, 1))
 #undef BVML_FFN_GO
     return hipGetLastError();
 }
@@ -248,7 +282,7 @@ hipError_t launch_norm_grad(const NormGradCall& c, hipStream_t s) {
 #define BVML_FFN_GO(T, V)                                                              \
     hipLaunchKernelGGL((norm_grad_kernel<T, V>), dim3((unsigned)blocks),               \
                        dim3(T == 64 ? 256 : T), 0, s, c);
-        BVML_FFN_TEAMS(BVML_FFN_GO)
+        BVML_FFN_TEAMS(BVML_FFN_GO, BVML_FFN_GO(64, 2))
 #undef BVML_FFN_GO
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

@@ -18,15 +18,16 @@ __device__ __forceinline__ void column_sum(const ColumnSum& c, int block, float 
     float t = 0.0f;
     if (col < c.cols) {
         const float* p = c.part + col;
-        int r = y;
-        for (; r + (kInFlight - 1) * kRuns < c.parts; r += kInFlight * kRuns) {
+        for (int r = y; r < c.parts; r += kInFlight * kRuns) {
             float v[kInFlight];
 #pragma unroll
-            for (int i = 0; i < kInFlight; ++i) v[i] = p[(long long)(r + i * kRuns) * c.cols];
+            for (int i = 0; i < kInFlight; ++i) {
+                const int at = r + i * kRuns;  // beyond the last: that one again, not added
+                v[i] = p[(long long)(at < c.parts ? at : c.parts - 1) * c.cols];
+            }
 #pragma unroll
-            for (int i = 0; i < kInFlight; ++i) t += v[i];
+            for (int i = 0; i < kInFlight; ++i) t += r + i * kRuns < c.parts ? v[i] : 0.0f;
         }
-        for (; r < c.parts; r += kRuns) t += p[(long long)r * c.cols];
     }
     sums[y][x] = t;
     __syncthreads();
