@@ -6,15 +6,23 @@
 //   input's       P = dz, k along its rows      Q = W,  k across its rows
 //   weight's      P = dz, k across its rows     Q = x,  k across its rows
 //
-// A workgroup of WM x WN waves owns a BM x BN tile of C; a wave its
-// (BM / WM) x (BN / WN) part, in fp32 accumulators of 32 x 32.  k goes by in
-// steps of 128 bytes (64 16-bit or 128 8-bit elements: whole cache lines of
-// every row), each multiplied in two halves.  Two LDS slots hold a step of
-// both operands each.  While a half is multiplied the next half's operands
-// are read from LDS into the other set of registers, and in a step's second
-// half, when every wave has read its slot, the step after the next is copied
-// over it; reads and copies are dealt out between the products, so that the
-// matrix cores never wait for a burst of them.  One barrier a step.
+// A workgroup of 2 x 2 waves owns a BM x BN tile of C; a wave a quarter of it,
+// in fp32 accumulators of 32 x 32.  k goes by in steps of 128 bytes (64 16-bit
+// or 128 8-bit elements: whole cache lines of every row), each multiplied in two
+// halves.  kSlots LDS slots hold a step of both operands each.  While a half is
+// multiplied the next half's operands are read from LDS into the other set of
+// registers, and in a step's second half, when every wave has read its slot,
+// the step kSlots later is copied over it; reads and copies are dealt out
+// between the products, so that the matrix cores never wait for a burst of
+// them.  One barrier a step.
+//
+// What bounds it: at 256 x 256 the matrix cores and the clock they leave
+// (4096 x 4096 x 8192 at 1350 TFLOP/s; one address for all rows, so that
+// nothing comes from memory, makes 4096 x 4096 x 5120 25% faster); at 128 x 128 the
+// way from cache to LDS, 64 bytes a clock and CU (1130); below that the latency of
+// a step.  4805 x 5120 x 1280, 380 tiles of 128 x 128, takes 66 us with its
+// operands in the caches and 80 without, 256 x 128 tiles with three slots
+// 64 to 75 and 83, 256 x 256 96 and 137.  8-bit 4805 x 1280 x 5120: 48 us.
 //
 // LDS layout, operand with k along its rows: 128 bytes a row, its eight
 // 16-byte pieces permuted by the row (piece ^ key) so that the rows a matrix

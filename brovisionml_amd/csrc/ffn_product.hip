@@ -1,5 +1,5 @@
-// Which kernel a product takes, the few-rows kernel, and the second launch
-// that joins a split sum.
+// Which kernel a product takes, the two kernels for few rows, and the second
+// launch that joins a split sum.
 
 #include "ffn_kernels.h"
 #include "ffn_product.h"
@@ -37,16 +37,21 @@ __device__ __forceinline__ v4i row_piece(const char* at, int k, int end) {
 }
 
 // ---------------------------------------------------------------------------
-// few rows (serving): the weights are read once, by workgroups of 8 or 16
+// few rows (5 to 32, serving): the weights are read once, by workgroups of 8
 // waves that share 16 rows of W (gated: 16 of each half) and divide k; their
 // sums meet in LDS.  Bound by reading W and, at these sizes, by the latency of
 // doing so: every lane has its 16-byte pieces of kAhead k groups in flight,
 // and what the epilogue adds is asked for first.  The matrix instruction's
-// other operand holds up to 16 rows of x, so a row costs what sixteen cost.
+// other operand holds up to 16 rows of x.  Every workgroup reads all of x, a
+// 64-byte run of a row at a time, which is what more rows cost.  Weights from
+// memory: 16 x 4096 x 4096 10.8 us, 3.1 TB/s; 16 x 1280 x 1280 4.7.  (16 waves:
+// 16 x 5120 x 1280 11.0 us for 11.2, 12 x 1024 x 1024 3.8 for 3.6: not kept.)
 // ---------------------------------------------------------------------------
-template <int kIn, int kBlocks, int kWaves, bool kGated, bool kWhole>
-__global__ __launch_bounds__(64 * kWaves) void rows_kernel(Product a) {
-    constexpr int kHalves = kGated ? 2 : 1;
+constexpr int kRowsWaves = 8;
+
+template <int kIn, int kBlocks, bool kGated, bool kWhole>
+__global__ __launch_bounds__(64 * kRowsWaves) void rows_kernel(Product a) {
+    constexpr int kHalves = kGated ? 2 : 1, kWaves = kRowsWaves;
     constexpr int kSize = kIn == kE4M3 ? 1 : 2, kPiece = 16 / kSize, kStep = 128 / kSize;
     constexpr int kAhead = kBlocks > 1 || kGated ? 2 : 5;
     __shared__ v4f sums[kWaves][kHalves][kBlocks][64];
@@ -130,7 +135,9 @@ __global__ __launch_bounds__(64 * kWaves) void rows_kernel(Product a) {
 // lanes their k, 16 adjacent bytes a lane, so that every load is whole cache
 // lines of one row and the work spreads over every CU.  Products and sums
 // are fp32 on the vector units: at so few rows the weights' way from memory
-// is all that counts.
+// is all that counts.  Weights from memory: 1 x 4096 x 4096 7.6 us, 4.4 TB/s;
+// 1 x 5120 x 1280 5.1.  The kernel above takes 7.7 for 4.6 with the latter in the
+// caches, and wins from 5 rows on (8 x 1280 x 5120: 6.1 us, this one 7.9).
 // ---------------------------------------------------------------------------
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
@@ -242,7 +249,9 @@ __global__ __launch_bounds__(256) void dot_kernel(Product a) {
 }
 
 // Sums the parts of the split tiles, in their order, and finishes them: a
-// thread 8 columns of a row, blockIdx.y the tile.
+// thread 8 columns of a row, blockIdx.y the tile.  Bound by memory and its own
+// launch: 4 tiles of 256 x 256 in 16 parts, 17 MB, 10 us.  The order is fixed,
+// so equal inputs give equal bits; atomic sums would not.
 template <bool kGated>
 __global__ __launch_bounds__(256) void join_kernel(Product a, int in_type, int bm, int bn) {
     const int cols = kGated ? bn / 2 : bn, per = cols / 8;
@@ -298,13 +307,13 @@ Product product_of(const ProductCall& c) {
     return a;
 }
 
-template <int kIn, int kBlocks, int kWaves, bool kGated>
+template <int kIn, int kBlocks, bool kGated>
 hipError_t launch_rows_one(const Product& a, bool whole, hipStream_t s) {
-    const dim3 grid((unsigned)((a.e.N + 15) / 16)), block(64 * kWaves);
+    const dim3 grid((unsigned)((a.e.N + 15) / 16)), block(64 * kRowsWaves);
     if (whole)
-        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kWaves, kGated, true>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kGated, true>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kWaves, kGated, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((rows_kernel<kIn, kBlocks, kGated, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
@@ -318,28 +327,23 @@ hipError_t launch_dot_one(const Product& a, bool whole, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int kIn, int kM, bool kGated>
-hipError_t launch_dot_of(const Product& a, bool whole, hipStream_t s) {
-    // two columns a wave once that leaves two workgroups a CU
-    return a.e.N >= 4096 ? launch_dot_one<kIn, kM, 2, kGated>(a, whole, s)
-                         : launch_dot_one<kIn, kM, 1, kGated>(a, whole, s);
-}
-
 template <int kIn, bool kGated>
 hipError_t launch_rows_of(const Product& a, bool whole, hipStream_t s) {
-    if (a.M == 1) return launch_dot_of<kIn, 1, kGated>(a, whole, s);
-    if (a.M == 2) return launch_dot_of<kIn, 2, kGated>(a, whole, s);
-    if (a.M <= 4) return launch_dot_of<kIn, 4, kGated>(a, whole, s);
-    if (a.M <= 16) {
-        // 16 waves where the workgroups are few and k is long enough for them
-        // (not for the gated form, whose sums do not fit their registers)
+    if (a.M == 1) return launch_dot_one<kIn, 1, 1, kGated>(a, whole, s);
+    if (a.M == 2) return launch_dot_one<kIn, 2, 1, kGated>(a, whole, s);
+    if (a.M <= 4) {
+        // A wave of two columns reads x half as often, and that is what counts
+        // from 3 rows on, once two workgroups a CU are left: 4 x 1280 x 8192 7.3
+        // to 6.3 us; 1 x 1280 x 5120 takes 4.3 either way, and 4 x 5120 x 2048 7.3
+        // for 6.5.  Gated waves have two columns as it is: four take 4 x 1280 x 5120
+        // from 7.3 to 7.6.
         if constexpr (!kGated) {
-            if (a.e.N <= 16 * 256 && a.steps >= 32)
-                return launch_rows_one<kIn, 1, 16, kGated>(a, whole, s);
+            if (a.e.N >= 4096) return launch_dot_one<kIn, 4, 2, kGated>(a, whole, s);
         }
-        return launch_rows_one<kIn, 1, 8, kGated>(a, whole, s);
+        return launch_dot_one<kIn, 4, 1, kGated>(a, whole, s);
     }
-    return launch_rows_one<kIn, 2, 8, kGated>(a, whole, s);
+    return a.M <= 16 ? launch_rows_one<kIn, 1, kGated>(a, whole, s)
+                     : launch_rows_one<kIn, 2, kGated>(a, whole, s);
 }
 
 hipError_t launch_rows(const ProductCall& c, hipStream_t s) {
@@ -393,7 +397,18 @@ double step_cost(const TileCost& c, double full) {
     const double over = 2.0 * full - 1.0;
     return c.idle + (c.step - c.idle) * (c.room > 256 ? 0.8 + 0.2 * over : over);
 }
-constexpr int kFewRows = 32;
+// The few-rows kernel: always up to kDotRows rows, possible up to kFewRows. Its
+// cost from 5 rows on, measured as above: rounds of a workgroup a CU, a step of
+// which takes longer with every row (16 x 4096 x 4096: 10.9 us, 32 rows 14.4).  The
+// tiles' costs are of operands that the caches hold; so few rows' weights
+// mostly come from memory, which takes a tile's first steps kCold longer.
+constexpr int kDotRows = 4, kFewRows = 32;
+constexpr double kCold = 1.2;
+double rows_cost(int M, int n, long long steps, bool gated) {
+    const double step = gated ? 0.15 + 0.0027 * M + (M > 16 ? 0.022 : 0.0)
+                              : 0.095 + 0.0024 * M + (M > 16 ? 0.015 : 0.0);
+    return (gated ? 2.75 : 2.5) + ceil_div(n, 16 * 256) * steps * step;
+}
 // A second launch, and a byte of a part written and read.
 constexpr double kJoin = 5.0, kJoinBytes = 8.0 / 4e6;
 
@@ -402,6 +417,12 @@ ProductPlan search_product(int M, int R, int K, int in_type, int layout, bool ga
     const long long steps = ceil_div(K, step_of(in_type));
     ProductPlan best{kTile128, dma, 0, 1};
     double least = 1e30;
+    if (layout == kForward && M <= kFewRows) {
+        // (without direct copies the tiles lose to it at all of these rows)
+        best = {kTileRows, dma, 0, 1};
+        if (!dma || M <= kDotRows) return best;
+        least = rows_cost(M, n, steps, gated) - kCold;
+    }
     for (int tile = kTile256; tile <= kTileSquare; ++tile) {
         if ((!dma && tile != kTile128) || (gated && tile == kTileSquare)) continue;
         const TileCost& c = kCosts[tile];
@@ -436,9 +457,7 @@ ProductPlan search_product(int M, int R, int K, int in_type, int layout, bool ga
 // and for its launch, and a search takes 0.4 us: a thread keeps its last
 // plans, by their sizes.)
 ProductPlan plan_product(int M, int R, int K, int in_type, int layout, bool gated, bool dma) {
-    // (every workgroup of the few-rows kernel reads all of x: 64 rows of 1,280 by
-    // 5,120 columns take it 15 us, the 64 x 64 tiles 7; 32 rows 8)
-    if (layout == kForward && M <= kFewRows) return {kTileRows, dma, 0, 1};
+    if (layout == kForward && M <= kDotRows) return {kTileRows, dma, 0, 1};
     struct Known {
         int M, R, K, kind;
         ProductPlan plan;

@@ -9,7 +9,7 @@ namespace bvml_ffn {
 // 32 columns a workgroup of 32 kRuns threads: kRuns interleaved runs of the
 // parts, each in its order, then the runs.  Bound by latency: a thread has
 // eight of its loads in flight (1,024 rows of 1,024 columns: 4.7 us; 39 with
-// one at a time).
+// one at a time; sixteen gain nothing), the last ones too.
 template <int kRuns>
 __device__ __forceinline__ void column_sum(const ColumnSum& c, int block, float (*sums)[32]) {
     constexpr int kInFlight = 8;
