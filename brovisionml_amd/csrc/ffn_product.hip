@@ -388,6 +388,11 @@ constexpr TileCost kCosts[] = {
     {64, 128, 512, 3.0, 0.55, 0.33, 0.12},   // 2048 x 1024 x 5120: 29 us, 34 with 64 x 64
     {64, 64, 512, 2.8, 0.40, 0.19, 0.09},    // 512 x 1280 x 5120: 18 us, 26 with 64 x 128
 };
+// The two of them that also copy through registers, then: a step's copies wait
+// for their loads (64 x 5120 x 1280: 22 us in one part, 64 x 64 tiles 15).
+constexpr TileCost kCopied128{128, 128, 512, 4.9, 1.20, 0.87, 0.03};
+constexpr TileCost kCopiedSquare{64, 64, 512, 3.3, 0.66, 0.58, 0.10};
+
 // With part of the card's room taken, 0 to 1.  Up to one workgroup a CU costs
 // `idle`; the first second one makes its CU the last to finish (64 x 64 tiles
 // of 5,120 terms: 256 of them 19 us, 384 33, 512 34).  Where one fills a CU, the
@@ -424,8 +429,11 @@ ProductPlan search_product(int M, int R, int K, int in_type, int layout, bool ga
         least = rows_cost(M, n, steps, gated) - kCold;
     }
     for (int tile = kTile256; tile <= kTileSquare; ++tile) {
-        if ((!dma && tile != kTile128) || (gated && tile == kTileSquare)) continue;
-        const TileCost& c = kCosts[tile];
+        if (gated && tile == kTileSquare) continue;
+        if (!dma && tile != kTile128 && tile != kTileSquare) continue;
+        const TileCost& c = dma                ? kCosts[tile]
+                            : tile == kTile128 ? kCopied128
+                                               : kCopiedSquare;
         const long long tiles = ceil_div(M, c.bm) * ceil_div(n, gated ? c.bn / 2 : c.bn);
         // rounds of a full card, then what is left over: one workgroup a tile
         // or, where that leaves CUs idle, several that share its terms

@@ -22,7 +22,12 @@ hipError_t launch_one(const Product& a, hipStream_t s) {
 
 template <int kIn, bool PT, bool QT, bool G>
 hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) {
-    if (!p.dma) return launch_one<kIn, 128, 128, 2, PT, QT, G, false>(a, s);
+    if (!p.dma) {
+        if constexpr (!G) {
+            if (p.tile == kTileSquare) return launch_one<kIn, 64, 64, 2, PT, QT, G, false>(a, s);
+        }
+        return launch_one<kIn, 128, 128, 2, PT, QT, G, false>(a, s);
+    }
     switch (p.tile) {
         case kTile256: return launch_one<kIn, 256, 256, 2, PT, QT, G, true>(a, s);
         case kTile128: return launch_one<kIn, 128, 128, 2, PT, QT, G, true>(a, s);

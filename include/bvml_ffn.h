@@ -143,13 +143,14 @@ long long bvml_ffn_gated_backward_workspace(int M, int N, int K);
 /*
  * The kernel a product of C (M, R) over K takes, without launching: *tile
  * receives its rows of C a workgroup (256, 128, 64; 0: the few-rows kernel),
- * *deep 1 for a tile with four LDS slots (128 x 128 and 64 x 64), *whole the tiles that one
- * workgroup sums, *splits the workgroups that share each of the others; any of
- * them may be NULL.  layout 0: the forward product (R = N, or 2N when gated),
- * 1: the input's gradient, 2: the weight's; 3: both at once from dz (M, R)
- * for x (M, K), *whole and *splits of the one whose sums are split.  aligned:
- * whether every operand row begins on 16 bytes and is whole pieces of them
- * (3: taken as given).  For tests and tuning.
+ * *deep 1 for the tiles with four LDS slots (128 x 128; 64 x 64, two without
+ * aligned), *whole the tiles that one workgroup sums, *splits the workgroups
+ * that share each of the others; any of them may be NULL.  layout 0: the
+ * forward product (R = N, or 2N when gated), 1: the input's gradient, 2: the
+ * weight's; 3: both at once from dz (M, R) for x (M, K), *whole and *splits of
+ * the one whose sums are split.  aligned: whether every operand row begins on
+ * 16 bytes and is whole pieces of them (3: taken as given).  For tests and
+ * tuning.
  */
 int bvml_ffn_plan(int M, int R, int K, int in_type, int layout, int gated, int aligned, int* tile,
                   int* deep, int* whole, int* splits);

@@ -204,7 +204,8 @@ def test_plan_reaches_every_kernel():
     want = {(0, False, a, False) for a in (True, False)}
     want |= {(256, False, True, False), (128, False, True, False), (128, True, True, False),
              (64, False, True, False), (64, False, True, True), (64, True, True, False),
-             (64, True, True, True), (128, False, False, False), (128, False, False, True)}
+             (64, True, True, True), (128, False, False, False), (128, False, False, True),
+             (64, True, False, False), (64, True, False, True)}
     assert want <= seen, want - seen
     seen = set()
     for M, N, K in t.GRADIENTS:
