@@ -277,7 +277,9 @@ def test_gradients_against_differences(cuda, name):
 # ---------------------------------------------------------------------------
 NORM = [(1, 1), (1, 1280), (3, 7), (5, 64), (130, 513), (9, 1024), (6, 1025), (77, 1536),
         (10, 1537), (5, 2048), (4, 2049), (3, 3000), (2, 4096), (3, 4097), (4, 6000), (7, 8192),
-        (2, 8195), (2, 20001), (1, 32768), (4805, 128)]
+        (2, 8195), (2, 20001), (1, 32768), (4805, 128),
+        # several rows a team, of three waves, five, and sixteen with more pieces
+        (5200, 1100), (2700, 2100), (600, 16500)]
 
 
 @pytest.mark.parametrize("xt,yt", [(BF, BF), (HF, HF), (FP, FP), (FP, BF), (FP, HF)])
