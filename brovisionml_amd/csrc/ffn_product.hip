@@ -249,11 +249,14 @@ __global__ __launch_bounds__(256) void dot_kernel(Product a) {
 }
 
 // Sums the parts of the split tiles, in their order, and finishes them: a
-// thread 8 columns of a row, blockIdx.y the tile.  Bound by memory and its own
-// launch: 4 tiles of 256 x 256 in 16 parts, 17 MB, 10 us.  The order is fixed,
-// so equal inputs give equal bits; atomic sums would not.
+// thread 8 columns of a row, blockIdx.y the tile.  Bound by latency, so eight
+// loads of parts are on their way together: 4 tiles of 256 x 256 in 16 parts 6 us,
+// 10 one part after another; 64 x 1280 in 10 parts 4.7 and 5.4 (gated, twice the
+// values a part: four parts 5.7, eight 7.4).  The order is fixed, so equal
+// inputs give equal bits; atomic sums would not.
 template <bool kGated>
 __global__ __launch_bounds__(256) void join_kernel(Product a, int in_type, int bm, int bn) {
+    constexpr int kHalves = kGated ? 2 : 1, kInFlight = 8 / kHalves;  // parts on their way
     const int cols = kGated ? bn / 2 : bn, per = cols / 8;
     const int t = blockIdx.x * 256 + threadIdx.x;
     const int row = t / per, col = t % per * 8;
@@ -266,20 +269,35 @@ __global__ __launch_bounds__(256) void join_kernel(Product a, int in_type, int b
     const int type16 = type16_of(in_type, a.e);
     Single<8, kGated> terms;
     terms.load(a.e, type16, m, n);
-    float v[8], u[8];
-    load_row<8>(from, kF32, 0, 8, v);
-    if constexpr (kGated) load_row<8>(from, kF32, cols, 8, u);
-    for (int s = 1; s < a.splits; ++s) {
-        from += bm * bn;
-        float x[8];
-        load_row<8>(from, kF32, 0, 8, x);
+    v4f sum[kHalves][2] = {};
+    for (int s = 0; s < a.splits; s += kInFlight) {
+        v4f x[kInFlight][kHalves][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += x[i];
-        if constexpr (kGated) {
-            load_row<8>(from, kF32, cols, 8, x);
+        for (int t = 0; t < kInFlight; ++t) {
+            // beyond the last: that one again, not added
+            const int at = s + t < a.splits ? s + t : a.splits - 1;
+            const v4f* const p = reinterpret_cast<const v4f*>(from + (long long)at * bm * bn);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] += x[i];
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[t][h][i] = p[h * (cols / 4) + i];
         }
+#pragma unroll
+        for (int t = 0; t < kInFlight; ++t) {
+            const bool in = s + t < a.splits;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[h][i][j] += in ? x[t][h][i][j] : 0.0f;
+        }
+    }
+    float v[8], u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        v[i] = sum[0][i / 4][i % 4];
+        u[i] = sum[kHalves - 1][i / 4][i % 4];
     }
     terms.finish(a.e, type16, m, n, v, u);
 }
