@@ -66,3 +66,75 @@ def test_e4m3_of_a_row_beyond_float32(cuda):
     others = torch.arange(64, device=cuda) != 3
     assert not got.y[1].float()[others].any() and got.y[[0, 2]].float().isfinite().all()
     assert (got.y[[0, 2], 3].float() == 448).all()
+
+
+# ---------------------------------------------------------------------------
+# activations: relative to their own value
+# ---------------------------------------------------------------------------
+ULP = 2.0 ** -24  # half a unit in the last place of fp32, relative
+
+
+def _reference(name, z):
+    """(act, its derivative) in double; each tail by itself, where it does not
+    cancel."""
+    if name == "gelu":
+        cdf = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+        return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if name == "gelu_tanh":
+        a = 2 * math.sqrt(2 / math.pi)
+        p = torch.sigmoid(a * (z + 0.044715 * z ** 3))
+        return z * p, p + z * p * (1 - p) * a * (1 + 3 * 0.044715 * z * z)
+    p = torch.sigmoid(z)
+    return z * p, p + z * p * (1 - p)
+
+
+def _relative(name, z):
+    """How far fp32 may be from act(z), relative to it, and the smallest value
+    that an fp32 tail can hold.
+
+    The tail is 2^t, and t's own roundings (its constants, products and
+    additions, five at most) are each |t| ln 2 ULP of it; then come an
+    exponential and a reciprocal of 2 ULP each (one unit), GELU's polynomial
+    (eight fused steps whose terms add up to less than twice its value: 16 ULP,
+    and 2 ULP of fit) and three products.  Below 2^-126 a factor of x may be
+    zero: |x| 2^-126, with |x| < 128."""
+    t = {"gelu": z * z / 2, "gelu_tanh": 1.6 * (z.abs() + 0.045 * z.abs() ** 3),
+         "silu": z.abs()}[name]
+    return (5 * t + 28) * ULP, 2.0 ** -119
+
+
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+def test_activation_tails_keep_their_relative_accuracy(cuda, name):
+    say(f"tails of {name}")
+    far = 90 if name == "silu" else 14
+    z = torch.cat([torch.linspace(-far, 14, 9001, device="cuda"),
+                   -torch.logspace(-6, 1, 301, device="cuda")]).to(BF)
+    got = ffn.linear(z[:, None], torch.ones(1, 1, device="cuda", dtype=BF), act=name,
+                     dtype=FP).y[:, 0].double()
+    z = z.double()
+    want, _ = _reference(name, z)
+    rel, floor = _relative(name, z)
+    bad = ~((got - want).abs() <= rel * want.abs() + floor)
+    worst = ((got - want).abs() / want.abs().clamp(min=floor)).max()
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}, {float(worst):.3g} relative"
+
+
+@pytest.mark.parametrize("name", ["gelu", "gelu_tanh", "silu"])
+def test_gated_gradient_keeps_the_tails(cuda, name):
+    """db of one row is [dh u act'(g), dh act(g)], rounded once to float16."""
+    say(f"gated gradient, tails of {name}")
+    g = torch.linspace(-6, 6, 4001, device="cuda").to(HF)[None]
+    n = g.shape[1]
+    x, w = torch.zeros(1, 8, device="cuda", dtype=HF), torch.zeros(2 * n, 8, device="cuda", dtype=HF)
+    dh = torch.full((1, n), 512.0, device="cuda", dtype=HF)
+    _, _, db = ffn.gated_backward(dh, x, w, torch.cat([g, torch.ones_like(g)], 1), name,
+                                  need_x=False, need_w=False)
+    value, slope = _reference(name, g[0].double())
+    rel, floor = _relative(name, g[0].double())
+    # the slope's two terms cancel near its root: relative to their sizes
+    size = slope.abs() + 2 * value.abs() * (1 + g[0].double().abs())
+    for got, want, off in ((db[:n], 512 * slope, 512 * rel * size),
+                           (db[n:], 512 * value, 512 * rel * value.abs())):
+        bound = off + 2.0 ** -11 * (want.abs() + off) + 2.0 ** -25 + 512 * floor
+        bad = ~((got.double() - want).abs() <= bound)
+        assert not bad.any(), int(bad.sum())
