@@ -162,7 +162,9 @@ __device__ __forceinline__ void act_slope1(int act, float x, float& value, float
             return;
         }
         case BVML_FFN_GELU_TANH: {
-            const float x2 = x * x, s = tanh_gate(x, x2);
+            // (s is 0 or 1 long before x^2 could pass the largest number, and
+            // 0 times that would be no number: the square stays below)
+            const float x2 = __builtin_fminf(x * x, 1e30f), s = tanh_gate(x, x2);
             value = x * s;
             slope = __builtin_fmaf(value * (1.0f - s),
                                    __builtin_fmaf(x2, 3.0f * kTanhA * kTanhB, kTanhA), s);

@@ -138,3 +138,22 @@ def test_gated_gradient_keeps_the_tails(cuda, name):
         bound = off + 2.0 ** -11 * (want.abs() + off) + 2.0 ** -25 + 512 * floor
         bad = ~((got.double() - want).abs() <= bound)
         assert not bad.any(), int(bad.sum())
+
+
+@pytest.mark.parametrize("name", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_of_the_largest_arguments(cuda, name):
+    """act' is 1 above and 0 below (none: 1) however large z is."""
+    say(f"largest arguments of {name}")
+    z = torch.tensor([s * 2.0 ** k for s in (1, -1) for k in range(6, 128)], device="cuda").to(BF)
+    n = len(z)
+    x, w = torch.zeros(1, 8, device="cuda", dtype=BF), torch.zeros(n, 8, device="cuda", dtype=BF)
+    dy = torch.ones(1, n, device="cuda", dtype=BF)
+    db = ffn.linear_backward(dy, x, w, z[None], name, need_x=False, need_w=False)[2].float()
+    want = torch.ones_like(db) if name == "none" else (z > 0).float()
+    # (2^6 is so far out that the tails are below 2^-60)
+    assert (db - want).abs().max() <= 2.0 ** -60
+    db = ffn.gated_backward(dy, x, torch.cat([w, w]), torch.cat([z, torch.ones_like(z)])[None],
+                            name, need_x=False, need_w=False)[2].float()
+    assert (db[:n] - want).abs().max() <= 2.0 ** -60
+    assert torch.equal(db[n:][want > 0], z.float()[want > 0])
+    assert not (db[n:][want == 0].abs() > 2.0 ** -60).any() and not db[n:].isnan().any()
