@@ -157,3 +157,48 @@ def test_slopes_of_the_largest_arguments(cuda, name):
     assert (db[:n] - want).abs().max() <= 2.0 ** -60
     assert torch.equal(db[n:][want > 0], z.float()[want > 0])
     assert not (db[n:][want == 0].abs() > 2.0 ** -60).any() and not db[n:].isnan().any()
+
+
+# ---------------------------------------------------------------------------
+# products of the smallest numbers, and of no numbers
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 7, 20, 40, 130, 300])
+def test_float16_subnormals_are_numbers(cuda, M):
+    """Integers times 2^-24 by small powers of two: every sum is exact."""
+    say(f"subnormals, {M} rows")
+    g = torch.Generator(device="cuda").manual_seed(M)
+    tiny = torch.randint(-1023, 1024, (48, 72), generator=g, device="cuda")
+    two = 2.0 ** torch.randint(0, 3, (M, 72), generator=g, device="cuda")
+    w, x = (tiny * 2.0 ** -24).to(HF), two.to(HF)
+    assert torch.equal(w.double(), tiny * 2.0 ** -24)
+    want = two.double() @ (tiny.double().t().contiguous() * 2.0 ** -24)
+    assert torch.equal(ffn.linear(x, w, dtype=FP).y.double(), want)
+    both = ffn.gated(x, torch.cat([w, torch.ones_like(w)]), act="none", dtype=FP).y.double()
+    assert torch.equal(both, want * two.double().sum(-1, keepdim=True))
+    # subnormal dz by rows of W and of x, results rounded once to float16
+    dz = (torch.randint(-1023, 1024, (M, 48), generator=g, device="cuda") * 2.0 ** -24).to(HF)
+    four = (2.0 ** torch.randint(0, 3, (48, 72), generator=g, device="cuda")).to(HF)
+    dx, dw, db = ffn.linear_backward(dz, x, four)
+    assert torch.equal(dx, (dz.double() @ four.double()).to(HF))
+    assert torch.equal(dw, (dz.double().t().contiguous() @ x.double()).to(HF))
+    assert torch.equal(db, dz.double().sum(0).to(HF))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, E4], ids=["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 17, 33, 150])
+def test_no_numbers_stay_in_their_rows(cuda, M, dtype):
+    say(f"NaN, {M} rows, {dtype}")
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn(M, 144, generator=g, device="cuda")
+    w = torch.randn(50, 144, generator=g, device="cuda")
+    x[M // 2, 131] = float("nan")
+    w[7, 5] = float("nan")
+    kw = {}
+    if dtype == E4:
+        kw = dict(x_scale=torch.ones(M, device="cuda"), w_scale=torch.ones(50, device="cuda"),
+                  dtype=FP)
+    y = ffn.linear(x.to(dtype), w.to(dtype), **kw).y
+    want = torch.zeros(M, 50, dtype=torch.bool, device="cuda")
+    want[M // 2] = True
+    want[:, 7] = True
+    assert torch.equal(y.isnan(), want)
