@@ -2,6 +2,7 @@
 // arguments, then the launches.  Nothing here allocates or synchronises.
 
 #include <cmath>
+#include <cstring>
 #include <initializer_list>
 #include <string>
 
@@ -48,10 +49,11 @@ int check_array(const std::string& op, const Array& a, bool optional) {
     return BVML_FFN_OK;
 }
 
-// No output may overlap an input or another output, but `same` may be `out`
-// itself, element for element.
+// No output may overlap an input or another output, but `may_out` may be any of
+// `may_in` itself, element for element.
 int check_alias(const std::string& op, std::initializer_list<Array> outs,
-                std::initializer_list<Array> ins, const char* may_out, const char* may_in) {
+                std::initializer_list<Array> ins, const char* may_out,
+                std::initializer_list<const char*> may_in) {
     const Array* o = outs.begin();
     for (size_t i = 0; i < outs.size(); ++i) {
         if (o[i].p == nullptr || o[i].bytes() == 0) continue;
@@ -60,9 +62,10 @@ int check_alias(const std::string& op, std::initializer_list<Array> outs,
                 return fail(BVML_FFN_EALIAS, op + ": " + o[i].name + " overlaps " + o[j].name);
         for (const Array& in : ins) {
             if (in.p == nullptr || !bvml::overlaps(o[i].p, o[i].bytes(), in.p, in.bytes())) continue;
-            const bool may = may_out && std::string(may_out) == o[i].name &&
-                             std::string(may_in).find(in.name) != std::string::npos &&
-                             in.p == o[i].p && in.ld == o[i].ld && in.type == o[i].type;
+            bool may = false;
+            if (may_out && std::strcmp(may_out, o[i].name) == 0 && in.p == o[i].p &&
+                in.ld == o[i].ld && in.type == o[i].type)
+                for (const char* name : may_in) may = may || std::strcmp(name, in.name) == 0;
             if (!may) return fail(BVML_FFN_EALIAS, op + ": " + o[i].name + " overlaps " + in.name);
         }
     }
@@ -128,7 +131,7 @@ int forward(const std::string& op, bool gated, const void* x, long long ldx, con
     BVML_FFN_TRY(check_array(op, ar, true));
     BVML_FFN_TRY(check_array(op, ay, false));
     BVML_FFN_TRY(check_array(op, az, true));
-    BVML_FFN_TRY(check_alias(op, {ay, az}, {ax, aw, ar, ab, axs, aws}, "y", "residual"));
+    BVML_FFN_TRY(check_alias(op, {ay, az}, {ax, aw, ar, ab, axs, aws}, "y", {"residual"}));
     if (M == 0) return BVML_FFN_OK;
     const long long need = product_workspace(M, (int)R, K, in_type, kForward, gated);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
@@ -190,14 +193,14 @@ int backward(const std::string& op, bool gated, const void* dy, long long lddy, 
     BVML_FFN_TRY(check_array(op, az, !sloped));
     BVML_FFN_TRY(check_array(op, adx, true));
     BVML_FFN_TRY(check_array(op, adw, true));
-    BVML_FFN_TRY(check_alias(op, {adx, adw, adb}, {ady, ax, aw, az}, nullptr, nullptr));
+    BVML_FFN_TRY(check_alias(op, {adx, adw, adb}, {ady, ax, aw, az}, nullptr, {}));
     if (!dx && !dw && !db) return BVML_FFN_OK;
     const GradSpace space(M, R, K, type);
     if (space.all() > 0 && (workspace == nullptr || workspace_bytes < space.all()))
         return fail(BVML_FFN_EWORK, op + ": the workspace must hold " +
                                         std::to_string(space.all()) + " bytes");
     const Array awork{"the workspace", workspace, space.all(), 1, space.all(), kE4M3};
-    BVML_FFN_TRY(check_alias(op, {awork}, {ady, ax, aw, az, adx, adw, adb}, nullptr, nullptr));
+    BVML_FFN_TRY(check_alias(op, {awork}, {ady, ax, aw, az, adx, adw, adb}, nullptr, {}));
     if (((uintptr_t)workspace & 15) != 0)
         return fail(BVML_FFN_EWORK, op + ": the workspace must begin on 16 bytes");
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -287,7 +290,7 @@ int bvml_ffn_add_rms_norm(const void* x, long long ldx, const void* residual, lo
     BVML_FFN_TRY(check_array(op, ar, true));
     BVML_FFN_TRY(check_array(op, ay, false));
     BVML_FFN_TRY(check_array(op, as, true));
-    BVML_FFN_TRY(check_alias(op, {ay, as, ac, ad}, {ax, ar, aw}, "stream", "x residual"));
+    BVML_FFN_TRY(check_alias(op, {ay, as, ac, ad}, {ax, ar, aw}, "stream", {"x", "residual"}));
     if (rows == 0) return BVML_FFN_OK;
     const NormCall c{x, residual, weight, ldx, ldr, ldy, lds, rows, cols, (float)eps, x_type,
                      w_type, y_type, y, stream_out, scale, rstd};
@@ -322,13 +325,13 @@ int bvml_ffn_add_rms_norm_backward(const void* dy, long long lddy, const void* s
     if (rows > 0 && rstd == nullptr) return fail(BVML_FFN_ENULL, op + ": rstd is NULL");
     BVML_FFN_TRY(check_array(op, adst, true));
     BVML_FFN_TRY(check_array(op, ads, false));
-    BVML_FFN_TRY(check_alias(op, {ads, adw}, {ady, as, aw, ar, adst}, "ds", "dstream"));
+    BVML_FFN_TRY(check_alias(op, {ads, adw}, {ady, as, aw, ar, adst}, "ds", {"dstream"}));
     const long long need = dweight ? norm_grad_workspace(rows, cols) : 0;
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(BVML_FFN_EWORK, op + ": the workspace must hold " + std::to_string(need) +
                                         " bytes");
     const Array awork{"the workspace", workspace, need, need > 0, need, kE4M3};
-    BVML_FFN_TRY(check_alias(op, {awork}, {ady, as, aw, ar, adst, ads, adw}, nullptr, nullptr));
+    BVML_FFN_TRY(check_alias(op, {awork}, {ady, as, aw, ar, adst, ads, adw}, nullptr, {}));
     const NormGradCall c{dy, s, weight, rstd, dstream, lddy, lds, lddst, ldds, rows, cols, dy_type,
                          s_type, w_type, ds, dweight, static_cast<float*>(workspace)};
     return launched(op, launch_norm_grad(c, static_cast<hipStream_t>(stream)));
