@@ -137,6 +137,12 @@ int forward(const std::string& op, bool gated, const void* x, long long ldx, con
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
         return fail(BVML_FFN_EWORK, op + ": the workspace must hold " + std::to_string(need) +
                                         " bytes");
+    if (need > 0) {
+        const Array awork{"the workspace", workspace, need, 1, need, kE4M3};
+        BVML_FFN_TRY(check_alias(op, {awork}, {ax, aw, ar, ab, axs, aws, ay, az}, nullptr, {}));
+        if (((uintptr_t)workspace & 15) != 0)
+            return fail(BVML_FFN_EWORK, op + ": the workspace must begin on 16 bytes");
+    }
     ProductCall c{};
     c.p = x;
     c.q = w;

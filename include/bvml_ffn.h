@@ -20,6 +20,9 @@
  * Sums, statistics and activations are fp32 whatever the types; a result is
  * rounded once, to nearest even, when it is stored.
  *
+ * A workspace holds at least what the operator's *_workspace function says,
+ * overlaps no other argument and, but for the norm's, begins on 16 bytes.
+ *
  * Return value: 0 on success; a negative BVML_FFN_E* code for a rejected
  * argument (nothing is launched); a positive hipError_t value when the HIP
  * runtime reports an error at launch.  bvml_ffn_last_error() returns the
@@ -37,9 +40,9 @@ extern "C" {
 #define BVML_FFN_ESHAPE (-2)  /* a negative size, a width below 1 or rows closer than their width */
 #define BVML_FFN_ETYPE (-3)   /* a type or a mixture of types the operator does not take */
 #define BVML_FFN_ESIZE (-4)   /* a size beyond the kernels' index range */
-#define BVML_FFN_EALIAS (-5)  /* an output overlaps an input or another output */
+#define BVML_FFN_EALIAS (-5)  /* an output or the workspace overlaps another argument */
 #define BVML_FFN_EPARAM (-6)  /* eps negative or not finite, an unknown activation */
-#define BVML_FFN_EWORK (-7)   /* the workspace is missing or too small */
+#define BVML_FFN_EWORK (-7)   /* the workspace is missing, too small or not on 16 bytes */
 
 /* Element types. */
 #define BVML_FFN_F32 0

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 
 from brovisionml_amd import _lib
-from tests.test_ffn_host import B, R, S, T, WORK, X, Y, Z, norm, norm_grad, product  # noqa: F401
+from tests.test_ffn_host import B, R, S, T, W, WORK, X, Y, Z, norm, norm_grad, product
 
 
 # ---------------------------------------------------------------------------
@@ -36,3 +36,35 @@ def test_the_named_aliases_pass_their_check():
 def test_norm_refuses_other_aliases(kw, message):
     assert norm(**kw) == _lib.FFN_EALIAS
     assert _lib.ffn_last_error() == "add_rms_norm: " + message
+
+
+# ---------------------------------------------------------------------------
+# the forward products' workspace, where their sums are split
+# ---------------------------------------------------------------------------
+SPLIT = dict(M=128, N=64, K=8192, ldx=8192, ldw=8192, ldy=64, ldr=64, ldz=128, it=_lib.BF16)
+
+
+@pytest.mark.parametrize("gated,at,name", [(False, R, "residual")] + [
+    (gated, at, name) for gated in (False, True)
+    for at, name in ((X + 4096, "x"), (W, "w"), (W + 1024 * 1024 - 16, "w"), (B, "bias"),
+                     (Y + 16, "y"), (Z, "z"))])
+def test_forward_refuses_a_workspace_over_another_argument(gated, at, name):
+    assert _lib.load_ffn().bvml_ffn_linear_workspace(128, 64, 8192, _lib.BF16) > 0
+    assert _lib.load_ffn().bvml_ffn_gated_workspace(128, 64, 8192, _lib.BF16) > 0
+    assert product(gated, work=at, **SPLIT) == _lib.FFN_EALIAS
+    name = "h" if gated and name == "y" else name
+    assert _lib.ffn_last_error().endswith(f": the workspace overlaps {name}")
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
+def test_forward_refuses_a_workspace_off_16_bytes(gated):
+    assert product(gated, work=WORK + 8, **SPLIT) == _lib.FFN_EWORK
+    assert "16 bytes" in _lib.ffn_last_error()
+
+
+@pytest.mark.parametrize("name,at", [("x_scale", S), ("w_scale", T)])
+def test_forward_refuses_a_workspace_over_the_scales(name, at):
+    kw = {**SPLIT, "it": _lib.E4M3, "K": 16384, "ldx": 16384, "ldw": 16384}
+    assert _lib.load_ffn().bvml_ffn_linear_workspace(128, 64, 16384, _lib.E4M3) > 0
+    assert product(work=at, xs=S, ws=T, z=0, **kw) == _lib.FFN_EALIAS
+    assert _lib.ffn_last_error() == f"linear: the workspace overlaps {name}"
