@@ -66,6 +66,7 @@ _VALUES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _li
 _HALVES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _OPERANDS = {**_HALVES, torch.float8_e4m3fn: _lib.E4M3}
 _F32 = torch.float32
+_MOST = 2 ** 31 - 1  # what the C entry points' sizes hold
 
 
 def _rows(op: str, name: str, t):
@@ -88,6 +89,8 @@ def _rows(op: str, name: str, t):
             elif s != step * rows:
                 _fail(f"{op}: {name}'s leading dimensions must collapse to evenly spaced rows")
             rows *= n
+    if rows > _MOST or cols > _MOST:
+        _fail(f"{op}: {name} has {rows} rows of {cols}, more than {_MOST} of either")
     if cols > 1 and stride[-1] != 1:
         _fail(f"{op}: {name}'s last dimension must be contiguous")
     # one row (or none) may be any distance from the next

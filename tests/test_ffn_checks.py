@@ -3,8 +3,9 @@ without a GPU: every call here fails its checks, or would before it could launch
 from __future__ import annotations
 
 import pytest
+import torch
 
-from brovisionml_amd import _lib
+from brovisionml_amd import _lib, ffn
 from tests.test_ffn_host import B, R, S, T, W, WORK, X, Y, Z, norm, norm_grad, product
 
 
@@ -68,3 +69,19 @@ def test_forward_refuses_a_workspace_over_the_scales(name, at):
     assert _lib.load_ffn().bvml_ffn_linear_workspace(128, 64, 16384, _lib.E4M3) > 0
     assert product(work=at, xs=S, ws=T, z=0, **kw) == _lib.FFN_EALIAS
     assert _lib.ffn_last_error() == f"linear: the workspace overlaps {name}"
+
+
+# ---------------------------------------------------------------------------
+# sizes beyond the entry points' 32-bit integers
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("shape", [(2 ** 32 + 5, 1), (2 ** 31, 8), (2 ** 16, 2 ** 16, 3),
+                                   (4, 2 ** 31), (2 ** 31,)])
+def test_sizes_beyond_32_bits_are_refused(shape):
+    t = torch.empty(shape, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(RuntimeError, match="ffn ops: op: x has .* more than 2147483647"):
+        ffn._rows("op", "x", t)
+
+
+def test_the_largest_sizes_are_taken():
+    t = torch.empty(2 ** 31 - 1, 1, dtype=torch.bfloat16, device="meta")
+    assert ffn._rows("op", "x", t) == (2 ** 31 - 1, 1, 1)
