@@ -266,8 +266,8 @@ int grad_blocks(int rows, int cols) {
                      : waves <= 16 ? 2
                                    : 1;
     const int most = 256 * each;
-    const int teams = waves <= 2 ? (rows + 3) / 4 : rows;
-    return teams < most ? teams : most;
+    const long long teams = waves <= 2 ? (rows + 3LL) / 4 : rows;
+    return teams < most ? (int)teams : most;
 }
 
 }  // namespace

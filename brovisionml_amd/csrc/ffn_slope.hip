@@ -34,7 +34,8 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeCall c, int rows_each) 
     const int n = (blockIdx.x * kLanes + x) * kVec, left = c.N - n;
     const int R = kGated ? 2 * c.N : c.N;
     const int r0 = blockIdx.y * rows_each;
-    const int r1 = r0 + rows_each < c.rows ? r0 + rows_each : c.rows;
+    // (the last run's end may be beyond what an int holds)
+    const int r1 = c.rows - r0 < rows_each ? c.rows : r0 + rows_each;
     float s[kHalves][kVec];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h)
@@ -118,10 +119,15 @@ __global__ __launch_bounds__(32 * kSumRuns) void column_sum_kernel(ColumnSum c) 
     column_sum<kSumRuns>(c, blockIdx.x, sums);
 }
 
-int rows_each_of(int rows) {
-    const int each = (rows + kMostParts - 1) / kMostParts;
-    const int whole = (each + kRows - 1) / kRows * kRows;
+// (in 64 bits: rows may be close to the largest int)
+long long rows_each_of(long long rows) {
+    const long long each = (rows + kMostParts - 1) / kMostParts;
+    const long long whole = (each + kRows - 1) / kRows * kRows;
     return whole < 16 ? 16 : whole;
+}
+int parts_of(long long rows) {
+    const long long each = rows_each_of(rows);
+    return (int)((rows + each - 1) / each);
 }
 
 }  // namespace
@@ -133,12 +139,11 @@ hipError_t launch_column_sum(const ColumnSum& c, hipStream_t s) {
 }
 
 long long slope_workspace(int rows, int R) {
-    const int each = rows_each_of(rows);
-    return (long long)((rows + each - 1) / each) * R * 4;
+    return (long long)parts_of(rows) * R * 4;
 }
 
 hipError_t launch_slope(const SlopeCall& c, ColumnSum* sums, hipStream_t s) {
-    const int each = rows_each_of(c.rows), parts = (c.rows + each - 1) / each;
+    const int each = (int)rows_each_of(c.rows), parts = parts_of(c.rows);
     const int R = c.gated ? 2 * c.N : c.N;
     *sums = {c.workspace, parts, R, c.db, c.type};
     if (parts == 0) return hipSuccess;

@@ -85,3 +85,14 @@ def test_sizes_beyond_32_bits_are_refused(shape):
 def test_the_largest_sizes_are_taken():
     t = torch.empty(2 ** 31 - 1, 1, dtype=torch.bfloat16, device="meta")
     assert ffn._rows("op", "x", t) == (2 ** 31 - 1, 1, 1)
+
+
+def test_workspaces_of_the_most_rows():
+    """dz is 16 bytes a row for one output, the rest the same for 256 runs of
+    rows, however close the rows are to the largest int."""
+    lib = _lib.load_ffn()
+    below, most = 2 ** 31 - 2 ** 23 - 2 ** 16, 2 ** 31 - 512
+    got = [lib.bvml_ffn_linear_backward_workspace(M, 1, 1) for M in (below, most)]
+    assert got[1] - got[0] == 16 * (most - below)
+    # 1,024 workgroups' partial rows
+    assert lib.bvml_ffn_add_rms_norm_backward_workspace(2 ** 31 - 1, 64) == 1024 * 64 * 4
