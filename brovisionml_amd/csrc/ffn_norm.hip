@@ -43,13 +43,21 @@ __device__ __forceinline__ T reduce(T v, Op op, T* slots) {
     return v;
 }
 
+// A launch holds fewer than 2^32 threads along x: workgroups beyond kMostX go
+// along y, and those beyond the last row return.
+constexpr long long kMostX = 1 << 20;
+dim3 grid_of(long long groups) {
+    if (groups <= kMostX) return dim3((unsigned)groups);
+    return dim3((unsigned)kMostX, (unsigned)((groups + kMostX - 1) / kMostX));
+}
+
 template <int kTeam, int kV>
 __global__ __launch_bounds__(kTeam == 64 ? 256 : kTeam) void norm_kernel(NormCall c) {
     __shared__ float sum_slots[kTeam / 64];
     __shared__ uint32_t max_slots[kTeam / 64];
     const int t = threadIdx.x % kTeam;
-    const long long row =
-        kTeam == 64 ? (long long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long long)blockIdx.x;
+    const long long group = (long long)blockIdx.y * kMostX + blockIdx.x;
+    const long long row = kTeam == 64 ? group * 4 + (threadIdx.x >> 6) : group;
     if (row >= c.rows) return;  // whole teams
     float v[kV][kVec];
     float sum = 0.0f;
@@ -274,8 +282,8 @@ int grad_blocks(int rows, int cols) {
 
 hipError_t launch_norm(const NormCall& c, hipStream_t s) {
     const int cols = c.cols;
-#define BVML_FFN_GO(T, V)                                                                   \
-    hipLaunchKernelGGL((norm_kernel<T, V>), dim3((unsigned)(T == 64 ? (c.rows + 3) / 4 : c.rows)), \
+#define BVML_FFN_GO(T, V)                                                                 \
+    hipLaunchKernelGGL((norm_kernel<T, V>), grid_of(T == 64 ? (c.rows + 3) / 4 : c.rows), \
                        dim3(T == 64 ? 256 : T), 0, s, c);
     BVML_FFN_TEAMS(BVML_FFN_GO, BVML_FFN_GO(128, 1))
 #undef BVML_FFN_GO

@@ -11,6 +11,12 @@ pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
 
+@pytest.fixture(autouse=True)
+def give_back():
+    yield
+    torch.cuda.empty_cache()
+
+
 def say(msg: str) -> None:
     print("[gpu] " + msg, flush=True)
 
@@ -26,3 +32,30 @@ def test_bias_gradient_of_the_most_rows(cuda):
     db = ffn.linear_backward(dy, z, torch.zeros(1, 1, dtype=BF, device=cuda), z, "silu",
                              need_x=False, need_w=False)[2]
     assert float(db) == 64.0  # silu'(0) = 1/2
+
+
+def _places(n: int, around: int):
+    """Indices below n: the first, the last, and those about multiples of
+    `around`."""
+    some = [torch.arange(min(n, 3000)), torch.arange(max(0, n - 3000), n)]
+    some += [torch.arange(k - 300, min(n, k + 300)) for k in range(around, n, around)]
+    return torch.cat(some).unique().cuda()
+
+
+# teams of one wave and of two, more rows than 2^32 threads have at once
+@pytest.mark.parametrize("rows,cols", [(2 ** 26 + 9, 8), (2 ** 25 + 3, 513)])
+def test_norm_of_more_rows_than_threads_along_a_grid(cuda, rows, cols):
+    say(f"norm {rows}x{cols}")
+    x = torch.empty(rows, cols, dtype=BF, device=cuda)
+    for part in x.split(2 ** 22):
+        part.normal_()
+    got = ffn.add_rms_norm(x, eps=1e-6, save=True)
+    at = _places(rows, 2 ** 22)
+    s = x[at].double()
+    want = s * torch.rsqrt((s * s).mean(-1, keepdim=True) + 1e-6)
+    off = (got.y[at].double() - want).abs()
+    assert (off <= want.abs() * (2.0 ** -8 + (cols + 16) * 2.0 ** -23)).all()
+    # every row was normed: its squares' mean is 1 but for y's rounding
+    for part in got.y.split(2 ** 22):
+        mean = part.float().square().mean(-1)
+        assert ((mean - 1).abs() <= 2.0 ** -6).all()
