@@ -80,6 +80,8 @@ int check_alias(const std::string& op, std::initializer_list<Array> outs,
 
 int launched(const std::string& op, hipError_t e) {
     if (e == hipSuccess) return BVML_FFN_OK;
+    if (e == hipErrorInvalidConfiguration)
+        return fail(BVML_FFN_ESIZE, op + ": more tiles than a launch holds");
     return fail((int)e, op + ": " + hipGetErrorString(e));
 }
 

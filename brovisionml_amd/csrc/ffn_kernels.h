@@ -6,6 +6,9 @@
 
 namespace bvml_ffn {
 
+// Workgroups of 256 threads that a launch holds: fewer than 2^32 threads.
+constexpr long long kMostGroups = (1LL << 24) - 1;
+
 // Which operand lies with k across its rows (ffn_product.h).
 enum Layout { kForward = 0, kInputGrad = 1, kWeightGrad = 2 };
 

@@ -629,6 +629,14 @@ struct Gradients {
     ColumnSum sums;
 };
 
+// Workgroups of a launch.
+inline long long groups_of(const Product& a) {
+    return a.whole + ((long long)a.tiles_m * a.tiles_n - a.whole) * a.splits;
+}
+inline long long groups_of(const Gradients& g) {
+    return groups_of(g.input) + groups_of(g.weight) + (g.sums.out ? (g.sums.cols + 31) / 32 : 0);
+}
+
 __device__ __forceinline__ int rest_of(const Product& a) {
     return (a.tiles_m * a.tiles_n - a.whole) * a.splits;
 }

@@ -552,7 +552,6 @@ hipError_t launch_product(const ProductCall& c, void* workspace, hipStream_t s) 
     if (p.tile == kTileRows) return launch_rows(c, s);
     Product a = product_of(c);
     lay_out(a, c, p.tile, p.whole, p.splits, workspace);
-    if ((long long)a.tiles_m * a.tiles_n > 0x7fffffffLL) return hipErrorInvalidConfiguration;
     const hipError_t e = c.in_type == kF16    ? launch_tiles_f16(a, p, c.layout, c.gated, s)
                          : c.in_type == kBF16 ? launch_tiles_bf16(a, p, c.layout, c.gated, s)
                                               : launch_tiles_e4m3(a, p, c.layout, c.gated, s);
@@ -676,19 +675,19 @@ long long gradients_workspace(int M, int R, int K) {
 
 hipError_t launch_gradients(const ProductCall& input, const ProductCall& weight,
                             const ColumnSum& sums, void* workspace, hipStream_t s) {
-    if (input.M == 0 || !dma_fits(input) || !dma_fits(weight)) {
+    auto apart = [&]() {
         hipError_t e = sums.out ? launch_column_sum(sums, s) : hipSuccess;
         if (e == hipSuccess && input.M > 0) e = launch_product(input, workspace, s);
         return e == hipSuccess ? launch_product(weight, workspace, s) : e;
-    }
+    };
+    if (input.M == 0 || !dma_fits(input) || !dma_fits(weight)) return apart();
     const GradientsPlan p = plan_gradients(input.M, input.K, input.R);
     Gradients g{product_of(input), product_of(weight), p.weight_first, sums};
     lay_out(g.input, input, p.tile, p.input_whole, p.input_splits, workspace);
     const long long ti = (long long)g.input.tiles_m * g.input.tiles_n;
     lay_out(g.weight, weight, p.tile, p.weight_whole, p.weight_splits,
             static_cast<char*>(workspace) + part_bytes(ti, p.input_whole, p.input_splits, p.tile));
-    if (ti > 0x7fffffffLL || (long long)g.weight.tiles_m * g.weight.tiles_n > 0x7fffffffLL)
-        return hipErrorInvalidConfiguration;
+    if (groups_of(g) > kMostGroups) return apart();
     hipError_t e = input.in_type == kF16 ? launch_gradients_f16(g, p.tile, s)
                                          : launch_gradients_bf16(g, p.tile, s);
     if (e == hipSuccess) e = join(g.input, input, p.tile, s);

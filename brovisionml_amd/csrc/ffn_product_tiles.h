@@ -3,8 +3,6 @@
 // a translation unit each so that they compile side by side.
 #pragma once
 
-#include <initializer_list>
-
 #include "ffn_kernels.h"
 #include "ffn_product.h"
 
@@ -12,9 +10,8 @@ namespace bvml_ffn {
 
 template <int kIn, int BM, int BN, int S, bool PT, bool QT, bool G, bool D>
 hipError_t launch_one(const Product& a, hipStream_t s) {
-    const long long rest = (long long)a.tiles_m * a.tiles_n - a.whole;
-    const long long groups = a.whole + rest * a.splits;
-    if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    const long long groups = groups_of(a);
+    if (groups > kMostGroups) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((product_kernel<kIn, BM, BN, S, PT, QT, G, D>), dim3((unsigned)groups),
                        dim3(256), 0, s, a);
     return hipGetLastError();
@@ -44,12 +41,8 @@ hipError_t launch_layout(const Product& a, const ProductPlan& p, hipStream_t s) 
 
 template <int kIn, int BM, int BN, int S>
 hipError_t launch_both(const Gradients& g, hipStream_t s) {
-    long long groups = g.sums.out ? (g.sums.cols + 31) / 32 : 0;
-    for (const Product* a : {&g.input, &g.weight})
-        groups += a->whole + ((long long)a->tiles_m * a->tiles_n - a->whole) * a->splits;
-    if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((gradients_kernel<kIn, BM, BN, S>), dim3((unsigned)groups), dim3(256), 0, s,
-                       g);
+    hipLaunchKernelGGL((gradients_kernel<kIn, BM, BN, S>), dim3((unsigned)groups_of(g)), dim3(256),
+                       0, s, g);
     return hipGetLastError();
 }
 

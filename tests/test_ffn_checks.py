@@ -96,3 +96,18 @@ def test_workspaces_of_the_most_rows():
     assert got[1] - got[0] == 16 * (most - below)
     # 1,024 workgroups' partial rows
     assert lib.bvml_ffn_add_rms_norm_backward_workspace(2 ** 31 - 1, 64) == 1024 * 64 * 4
+
+
+# ---------------------------------------------------------------------------
+# more tiles than one launch holds (2^32 threads)
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
+@pytest.mark.parametrize("N", [4096, 1 << 20])
+def test_more_tiles_than_a_launch_holds_are_refused(gated, N):
+    """Arrays of up to 2^52 bytes at addresses 2^56 apart: refused before any
+    launch."""
+    at = [(i + 1) << 56 for i in range(4)]
+    kw = dict(x=at[0], ldx=8, w=at[1], ldw=8, bias=0, residual=0, M=2 ** 31 - 512, N=N, K=8,
+              y=at[2], ldy=N, z=0, work=at[3], bytes=1 << 40)
+    assert product(gated, **kw) == _lib.FFN_ESIZE
+    assert "more tiles than a launch holds" in _lib.ffn_last_error()

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from brovisionml_amd import ffn
+from brovisionml_amd import _lib, ffn
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -59,3 +59,26 @@ def test_norm_of_more_rows_than_threads_along_a_grid(cuda, rows, cols):
     for part in got.y.split(2 ** 22):
         mean = part.float().square().mean(-1)
         assert ((mean - 1).abs() <= 2.0 ** -6).all()
+
+
+def test_both_gradients_of_more_tiles_than_a_launch_holds(cuda):
+    """2^30 + 77 rows are 2^24 + 2 tiles of the two gradients' common launch: each
+    then goes by itself.  Whole numbers, so that every sum is exact."""
+    rows, n, k = 2 ** 30 + 77, 8, 8
+    say(f"gradients of {rows} rows")
+    tile, deep, _, _ = _lib.ffn_plan(rows, n, k, _lib.BF16, 3)
+    assert (tile, deep) == (64, True) and (rows + 63) // 64 >= 2 ** 24
+    w = torch.randint(-4, 5, (n, k), device=cuda).to(BF)
+    x, dy = (torch.empty(rows, m, dtype=BF, device=cuda) for m in (k, n))
+    for part in (*x.split(2 ** 26), *dy.split(2 ** 26)):
+        part.random_(-1, 2)
+    dx, dw, db = ffn.linear_backward(dy, x, w)
+    want_w, want_b = 0, 0
+    for i in range(0, rows, 2 ** 25):
+        d, part = dy[i:i + 2 ** 25], slice(i, i + 2 ** 25)
+        # at most 8 products of up to 4, and 2^25 of up to 1: exact in fp32
+        assert torch.equal(dx[part].float(), d.float() @ w.float())
+        want_w = want_w + (d.float().t().contiguous() @ x[part].float()).double()
+        want_b = want_b + d.sum(0, dtype=torch.float32).double()
+    assert float(want_w.abs().max()) < 2 ** 23 and float(want_b.abs().max()) < 2 ** 23
+    assert torch.equal(dw, want_w.to(BF)) and torch.equal(db, want_b.to(BF))
