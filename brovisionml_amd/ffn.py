@@ -82,6 +82,9 @@ def _rows(op: str, name: str, t):
         cols = shape[-1]
         rows, step = 1, cols
         for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+            if n == 0:  # no rows, whatever the others' spacing
+                rows = 0
+                break
             if n == 1:
                 continue
             if rows == 1:

@@ -111,3 +111,11 @@ def test_more_tiles_than_a_launch_holds_are_refused(gated, N):
               y=at[2], ldy=N, z=0, work=at[3], bytes=1 << 40)
     assert product(gated, **kw) == _lib.FFN_ESIZE
     assert "more tiles than a launch holds" in _lib.ffn_last_error()
+
+
+@pytest.mark.parametrize("shape", [(3, 0, 64), (0, 5, 64), (3, 0, 2, 64), (2, 3, 0, 64), (0, 64)])
+def test_no_rows_in_any_dimension(shape):
+    t = torch.zeros(shape)
+    assert ffn._rows("op", "x", t)[:2] == (0, 64)
+    wide = torch.zeros(*shape[:-1], 100)[..., :64]
+    assert ffn._rows("op", "x", wide)[:2] == (0, 64)

@@ -82,3 +82,14 @@ def test_both_gradients_of_more_tiles_than_a_launch_holds(cuda):
         want_b = want_b + d.sum(0, dtype=torch.float32).double()
     assert float(want_w.abs().max()) < 2 ** 23 and float(want_b.abs().max()) < 2 ** 23
     assert torch.equal(dw, want_w.to(BF)) and torch.equal(db, want_b.to(BF))
+
+
+def test_no_rows_in_an_inner_dimension(cuda):
+    say("no rows")
+    x, w = torch.zeros(3, 0, 64, dtype=BF, device=cuda), torch.ones(40, 64, dtype=BF, device=cuda)
+    assert ffn.add_rms_norm(x, x).y.shape == x.shape
+    y = ffn.linear(x, w, save=True)
+    assert y.y.shape == y.z.shape == (3, 0, 40)
+    assert ffn.gated(x, w).y.shape == (3, 0, 20)
+    dx, dw, db = ffn.linear_backward(y.y, x, w)
+    assert dx.shape == x.shape and not dw.any() and not db.any()
