@@ -1,6 +1,6 @@
 // The usual call of a feed-forward operator from Python (brovisionml_amd/ffn.py):
-// contiguous tensors of one type on the current device, checked, given their
-// outputs and launched in C.  Anything out of the ordinary returns None, and
+// contiguous tensors of one type on the current device that autograd does not
+// record, checked, given their outputs and launched in C.  Anything out of the ordinary returns None, and
 // the Python function's own checks then take it or say what is wrong.  Against
 // the same steps in Python, time per call: a product of one row, 5120 to 1280,
 // 8.3-8.6 to 6.6-6.8 us; a norm of one row of 1280, 9.2-9.4 to 8.1-8.4 (both
@@ -18,9 +18,9 @@
 namespace {
 
 // what setup() hands over, kept for the process
-PyObject *g_f16, *g_bf16, *g_f32, *g_u8, *g_acts, *g_device, *g_stream;
+PyObject *g_f16, *g_bf16, *g_f32, *g_u8, *g_acts, *g_device, *g_stream, *g_recording;
 // method and attribute names
-PyObject *n_dtype, *n_device, *n_contiguous, *n_shape, *n_ptr, *n_empty;
+PyObject *n_dtype, *n_device, *n_contiguous, *n_shape, *n_ptr, *n_empty, *n_grad;
 
 struct Held {  // a reference that is given back
     PyObject* o;
@@ -46,7 +46,7 @@ constexpr int kMostDims = 8;
 struct Tensor {
     int type = -1;  // as type_of
     long device = -1;
-    bool contiguous = false;
+    bool contiguous = false, requires_grad = false;
     int dims = 0;
     Py_ssize_t shape[kMostDims];
     void* data = nullptr;
@@ -82,9 +82,19 @@ private:
         const Held ptr(PyObject_CallMethodNoArgs(t, n_ptr));
         if (!ptr.o) return false;
         data = PyLong_AsVoidPtr(ptr.o);
+        const Held grad(PyObject_GetAttr(t, n_grad));
+        requires_grad = grad.o == Py_True;
         return !PyErr_Occurred();
     }
 };
+
+// Whether autograd is to record a call on tensors of which some require a
+// gradient.
+bool recorded(bool any) {
+    if (!any) return false;
+    const Held on(PyObject_CallNoArgs(g_recording));
+    return on.o != Py_False;
+}
 
 // The current device is `index`, and its stream.
 bool stream_of(long index, void** stream) {
@@ -137,6 +147,8 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return unusual();
     if (has_residual && (!r.ask(args[4]) || r.type != x.type || r.device != x.device ||
                          !r.contiguous || r.dims != 2 || r.shape[0] != M || r.shape[1] != N))
+        return unusual();
+    if (recorded(x.requires_grad || w.requires_grad || b.requires_grad || r.requires_grad))
         return unusual();
     PyObject* const code = PyDict_GetItemWithError(g_acts, args[3]);
     void* stream = nullptr;
@@ -191,6 +203,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!w.ask(args[2]) || w.type != x.type || !w.contiguous || w.device != x.device ||
         w.numel() != cols)
         return unusual();
+    if (recorded(x.requires_grad || r.requires_grad || w.requires_grad)) return unusual();
     const double eps = PyFloat_AsDouble(args[3]);
     void* stream = nullptr;
     if (all < 1 || all / cols > (1 << 30) || cols > (1 << 30) || PyErr_Occurred() ||
@@ -210,14 +223,16 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyTuple_Pack(2, y.o, s.o);
 }
 
-// setup(float16, bfloat16, float32, uint8, acts, current_device, raw_stream)
+// setup(float16, bfloat16, float32, uint8, acts, current_device, raw_stream,
+// is_grad_enabled)
 PyObject* setup(PyObject*, PyObject* args) {
-    PyObject* o[7];
-    if (!PyArg_ParseTuple(args, "OOOOO!OO", &o[0], &o[1], &o[2], &o[3], &PyDict_Type, &o[4], &o[5],
-                          &o[6]))
+    PyObject* o[8];
+    if (!PyArg_ParseTuple(args, "OOOOO!OOO", &o[0], &o[1], &o[2], &o[3], &PyDict_Type, &o[4], &o[5],
+                          &o[6], &o[7]))
         return nullptr;
-    PyObject** const to[7] = {&g_f16, &g_bf16, &g_f32, &g_u8, &g_acts, &g_device, &g_stream};
-    for (int i = 0; i < 7; ++i) {
+    PyObject** const to[8] = {&g_f16,  &g_bf16,   &g_f32,    &g_u8,
+                              &g_acts, &g_device, &g_stream, &g_recording};
+    for (int i = 0; i < 8; ++i) {
         Py_INCREF(o[i]);
         Py_XDECREF(*to[i]);
         *to[i] = o[i];
@@ -232,7 +247,7 @@ PyMethodDef g_methods[] = {
     {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm)), METH_FASTCALL,
      "norm(x, residual, weight, eps, dtype): (y, stream), or None for an unusual call"},
     {"setup", setup, METH_VARARGS,
-     "setup(float16, bfloat16, float32, uint8, acts, current_device, raw_stream)"},
+     "setup(float16, bfloat16, float32, uint8, acts, current_device, raw_stream, is_grad_enabled)"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_ffn_call", nullptr, -1, g_methods,
@@ -246,7 +261,8 @@ PyMODINIT_FUNC PyInit__ffn_call(void) {
         const char* name;
     } const names[] = {{&n_dtype, "dtype"},       {&n_device, "get_device"},
                        {&n_contiguous, "is_contiguous"}, {&n_shape, "shape"},
-                       {&n_ptr, "data_ptr"},      {&n_empty, "new_empty"}};
+                       {&n_ptr, "data_ptr"},      {&n_empty, "new_empty"},
+                       {&n_grad, "requires_grad"}};
     for (const auto& n : names)
         if (!(*n.to = PyUnicode_InternFromString(n.name))) return nullptr;
     return PyModule_Create(&g_module);

@@ -16,6 +16,10 @@ products also take float8_e4m3fn operands with a float32 scale a row, as
 add_rms_norm(dtype=torch.float8_e4m3fn) leaves them.  Every call is
 asynchronous on the current stream of the tensors' device.
 
+Where autograd records (a tensor requires a gradient and gradients are enabled)
+add_rms_norm, linear and gated are recorded with these gradients; float8 and
+`out` then raise.  They are differentiable once.
+
 Errors raise RuntimeError with the "ffn ops: " prefix.
 """
 from __future__ import annotations
@@ -24,6 +28,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -58,7 +63,7 @@ def _fail(msg: str):
 def _call():
     module = _lib.load_ffn_call()
     module.setup(torch.float16, torch.bfloat16, torch.float32, torch.uint8, _ACTS, _device,
-                 _stream)
+                 _stream, torch.is_grad_enabled)
     return module
 
 
@@ -159,6 +164,14 @@ def _space(n: int, like):
     return t, t.data_ptr()
 
 
+def _recorded(*tensors) -> bool:
+    """Whether autograd is to record a call on these (some may be None)."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
+
+
 # ---------------------------------------------------------------------------
 # the norm
 # ---------------------------------------------------------------------------
@@ -174,6 +187,15 @@ def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, *, dtype=None
         done = _call().norm(x, residual, weight, eps, dtype)
         if done is not None:
             return Norm(done[0], None, done[1], None)
+    if _recorded(x, residual, weight):
+        if dtype == torch.float8_e4m3fn:
+            _fail("add_rms_norm: float8 output has no gradient: call it under torch.no_grad()")
+        y, rstd, *stream = _RecordedNorm.apply(eps, dtype, x, residual, weight)
+        return Norm(y, None, stream[0] if stream else x, rstd if save else None)
+    return _norm(x, residual, weight, eps, dtype, save)
+
+
+def _norm(x, residual, weight, eps, dtype, save) -> Norm:
     op = "add_rms_norm"
     index, xd = _index(op, x), x.dtype
     xt = _type(op, "x", xd, _VALUES)
@@ -201,6 +223,27 @@ def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, *, dtype=None
     _launch(op, index, _lib.load_ffn().bvml_ffn_add_rms_norm, x.data_ptr(), ldx, rp, ldr, wp, rows,
             cols, eps, xt, wt, yt, y.data_ptr(), cols, sp, cols, cp, dp)
     return Norm(y, scale, stream, rstd)
+
+
+class _RecordedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, eps, dtype, x, residual, weight):
+        n = _norm(x, residual, weight, eps, dtype, True)
+        ctx.save_for_backward(n.stream, weight, n.rstd)
+        ctx.y_shape, ctx.y_type = n.y.shape, n.y.dtype
+        ctx.mark_non_differentiable(n.rstd)
+        ctx.set_materialize_grads(False)
+        return (n.y, n.rstd) if residual is None else (n.y, n.rstd, n.stream)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _, dstream=None):
+        stream, weight, rstd = ctx.saved_tensors
+        dy = stream.new_zeros(ctx.y_shape, dtype=ctx.y_type) if dy is None else dy.contiguous()
+        ds, dw = add_rms_norm_backward(dy, stream, weight, rstd,
+                                       None if dstream is None else dstream.contiguous(),
+                                       need_weight=ctx.needs_input_grad[4])
+        return None, None, ds, ds if ctx.needs_input_grad[3] else None, dw
 
 
 def add_rms_norm_backward(dy, stream, weight, rstd, dstream=None, *, need_weight: bool = True):
@@ -315,7 +358,7 @@ def linear(x, w, bias=None, act: str = "none", residual=None, *, x_scale=None, w
         y = _call().product(x, w, bias, act, residual, False, dtype)
         if y is not None:
             return Product(y, None)
-    return _forward("linear", False, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out)
+    return _product("linear", False, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out)
 
 
 def gated(x, w, bias=None, act: str = "silu", *, x_scale=None, w_scale=None, dtype=None,
@@ -327,7 +370,45 @@ def gated(x, w, bias=None, act: str = "silu", *, x_scale=None, w_scale=None, dty
         y = _call().product(x, w, bias, act, None, True, dtype)
         if y is not None:
             return Product(y, None)
-    return _forward("gated", True, x, w, bias, act, None, x_scale, w_scale, dtype, save, out)
+    return _product("gated", True, x, w, bias, act, None, x_scale, w_scale, dtype, save, out)
+
+
+def _product(op: str, gated: bool, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out):
+    if not _recorded(x, w, bias, residual, x_scale, w_scale, out):
+        return _forward(op, gated, x, w, bias, act, residual, x_scale, w_scale, dtype, save, out)
+    if x.dtype == torch.float8_e4m3fn or x_scale is not None or w_scale is not None:
+        _fail(f"{op}: float8 operands have no gradient: call it under torch.no_grad()")
+    if out is not None:
+        _fail(f"{op}: a given output has no gradient: call it under torch.no_grad()")
+    return Product(*_RecordedProduct.apply(op, gated, act, dtype, save, x, w, bias, residual))
+
+
+class _RecordedProduct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, op, gated, act, dtype, save, x, w, bias, residual):
+        sloped = gated or act != "none"
+        y, z = _forward(op, gated, x, w, bias, act, residual, None, None, dtype, save or sloped,
+                        None)
+        ctx.save_for_backward(x, w, z if sloped else None)
+        ctx.call, ctx.bias = (op + "_backward", gated), bias is not None and (bias.shape, bias.dtype)
+        ctx.act = act
+        if not save:
+            return y, None
+        ctx.mark_non_differentiable(z)
+        return y, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _):
+        x, w, z = ctx.saved_tensors
+        need_x, need_w, need_bias, need_residual = ctx.needs_input_grad[5:]
+        op, gated = ctx.call
+        dx, dw, db = _backward(op, gated, dy.contiguous(), x, w, z, ctx.act, need_x, need_w,
+                               need_bias)
+        if need_bias:
+            shape, dtype = ctx.bias
+            db = db.reshape(shape).to(dtype)
+        return None, None, None, None, None, dx, dw, db, dy if need_residual else None
 
 
 def _backward(op: str, is_gated: bool, dy, x, w, z, act, need_x, need_w, need_bias):
