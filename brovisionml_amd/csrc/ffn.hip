@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
+#include <new>
 #include <string>
 
 #include "bvml_ffn.h"
@@ -61,7 +62,7 @@ int check_alias(const std::string& op, std::initializer_list<Array> outs,
             if (o[j].p && bvml::overlaps(o[i].p, o[i].bytes(), o[j].p, o[j].bytes()))
                 return fail(BVML_FFN_EALIAS, op + ": " + o[i].name + " overlaps " + o[j].name);
         for (const Array& in : ins) {
-            if (in.p == nullptr || !bvml::overlaps(o[i].p, o[i].bytes(), in.p, in.bytes())) continue;
+            if (!in.p || !bvml::overlaps(o[i].p, o[i].bytes(), in.p, in.bytes())) continue;
             bool may = false;
             if (may_out && std::strcmp(may_out, o[i].name) == 0 && in.p == o[i].p &&
                 in.ld == o[i].ld && in.type == o[i].type)
@@ -83,6 +84,17 @@ int launched(const std::string& op, hipError_t e) {
     if (e == hipErrorInvalidConfiguration)
         return fail(BVML_FFN_ESIZE, op + ": more tiles than a launch holds");
     return fail((int)e, op + ": " + hipGetErrorString(e));
+}
+
+// An entry point's body: nothing is thrown past it.  (What can be thrown is that
+// a message's memory is not there; the last message then stays.)
+template <typename F>
+int guarded(F body) noexcept {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return (int)hipErrorOutOfMemory;
+    }
 }
 
 int check_act(const std::string& op, int act) {
@@ -275,34 +287,39 @@ int bvml_ffn_add_rms_norm(const void* x, long long ldx, const void* residual, lo
                           const void* weight, int rows, int cols, double eps, int x_type,
                           int w_type, int y_type, void* y, long long ldy, void* stream_out,
                           long long lds, float* scale, float* rstd, void* stream) {
-    const std::string op = "add_rms_norm";
-    if (rows < 0 || cols < 1) return fail(BVML_FFN_ESHAPE, op + ": rows must be >= 0, cols >= 1");
-    if (cols > kMostNormCols) return fail(BVML_FFN_ESIZE, op + ": more than 32768 columns");
-    if (rows > kMostRows) return fail(BVML_FFN_ESIZE, op + ": too many rows");
-    if (!(eps >= 0.0) || !std::isfinite(eps))
-        return fail(BVML_FFN_EPARAM, op + ": eps must be finite and >= 0");
-    if (!is_value(x_type)) return fail(BVML_FFN_ETYPE, op + ": x must be f32, f16 or bf16");
-    if (weight && w_type != kF32 && w_type != x_type)
-        return fail(BVML_FFN_ETYPE, op + ": the weight must be f32 or of x's type");
-    if (y_type != x_type && y_type != kE4M3 && !(x_type == kF32 && is16(y_type)))
-        return fail(BVML_FFN_ETYPE, op + ": y must be of x's type, e4m3, or (from f32) 16 bits");
-    if ((y_type == kE4M3) != (scale != nullptr) && !(rows == 0 && scale == nullptr))
-        return fail(scale ? BVML_FFN_ETYPE : BVML_FFN_ENULL,
-                    op + ": e4m3 output, and no other, comes with scale");
-    const Array ax{"x", x, ldx, rows, cols, x_type}, ar{"residual", residual, ldr, rows, cols, x_type};
-    const Array aw{"weight", weight, cols, 1, cols, w_type};
-    const Array ay{"y", y, ldy, rows, cols, y_type};
-    const Array as{"stream", stream_out, lds, rows, cols, x_type};
-    const Array ac{"scale", scale, rows, 1, rows, kF32}, ad{"rstd", rstd, rows, 1, rows, kF32};
-    BVML_FFN_TRY(check_array(op, ax, false));
-    BVML_FFN_TRY(check_array(op, ar, true));
-    BVML_FFN_TRY(check_array(op, ay, false));
-    BVML_FFN_TRY(check_array(op, as, true));
-    BVML_FFN_TRY(check_alias(op, {ay, as, ac, ad}, {ax, ar, aw}, "stream", {"x", "residual"}));
-    if (rows == 0) return BVML_FFN_OK;
-    const NormCall c{x, residual, weight, ldx, ldr, ldy, lds, rows, cols, (float)eps, x_type,
-                     w_type, y_type, y, stream_out, scale, rstd};
-    return launched(op, launch_norm(c, static_cast<hipStream_t>(stream)));
+    return guarded([&]() -> int {
+        const std::string op = "add_rms_norm";
+        if (rows < 0 || cols < 1)
+            return fail(BVML_FFN_ESHAPE, op + ": rows must be >= 0, cols >= 1");
+        if (cols > kMostNormCols) return fail(BVML_FFN_ESIZE, op + ": more than 32768 columns");
+        if (rows > kMostRows) return fail(BVML_FFN_ESIZE, op + ": too many rows");
+        if (!(eps >= 0.0) || !std::isfinite(eps))
+            return fail(BVML_FFN_EPARAM, op + ": eps must be finite and >= 0");
+        if (!is_value(x_type)) return fail(BVML_FFN_ETYPE, op + ": x must be f32, f16 or bf16");
+        if (weight && w_type != kF32 && w_type != x_type)
+            return fail(BVML_FFN_ETYPE, op + ": the weight must be f32 or of x's type");
+        if (y_type != x_type && y_type != kE4M3 && !(x_type == kF32 && is16(y_type)))
+            return fail(BVML_FFN_ETYPE,
+                        op + ": y must be of x's type, e4m3, or (from f32) 16 bits");
+        if ((y_type == kE4M3) != (scale != nullptr) && !(rows == 0 && scale == nullptr))
+            return fail(scale ? BVML_FFN_ETYPE : BVML_FFN_ENULL,
+                        op + ": e4m3 output, and no other, comes with scale");
+        const Array ax{"x", x, ldx, rows, cols, x_type};
+        const Array ar{"residual", residual, ldr, rows, cols, x_type};
+        const Array aw{"weight", weight, cols, 1, cols, w_type};
+        const Array ay{"y", y, ldy, rows, cols, y_type};
+        const Array as{"stream", stream_out, lds, rows, cols, x_type};
+        const Array ac{"scale", scale, rows, 1, rows, kF32}, ad{"rstd", rstd, rows, 1, rows, kF32};
+        BVML_FFN_TRY(check_array(op, ax, false));
+        BVML_FFN_TRY(check_array(op, ar, true));
+        BVML_FFN_TRY(check_array(op, ay, false));
+        BVML_FFN_TRY(check_array(op, as, true));
+        BVML_FFN_TRY(check_alias(op, {ay, as, ac, ad}, {ax, ar, aw}, "stream", {"x", "residual"}));
+        if (rows == 0) return BVML_FFN_OK;
+        const NormCall c{x, residual, weight, ldx, ldr, ldy, lds, rows, cols, (float)eps, x_type,
+                         w_type, y_type, y, stream_out, scale, rstd};
+        return launched(op, launch_norm(c, static_cast<hipStream_t>(stream)));
+    });
 }
 
 long long bvml_ffn_add_rms_norm_backward_workspace(int rows, int cols) {
@@ -314,35 +331,38 @@ int bvml_ffn_add_rms_norm_backward(const void* dy, long long lddy, const void* s
                                    long long lddst, int rows, int cols, int dy_type, int s_type,
                                    int w_type, void* ds, long long ldds, void* dweight,
                                    void* workspace, long long workspace_bytes, void* stream) {
-    const std::string op = "add_rms_norm_backward";
-    if (rows < 0 || cols < 1) return fail(BVML_FFN_ESHAPE, op + ": rows must be >= 0, cols >= 1");
-    if (cols > kMostNormCols) return fail(BVML_FFN_ESIZE, op + ": more than 32768 columns");
-    if (rows > kMostRows) return fail(BVML_FFN_ESIZE, op + ": too many rows");
-    if (!is_value(s_type) || !is_value(dy_type))
-        return fail(BVML_FFN_ETYPE, op + ": s and dy must be f32, f16 or bf16");
-    if ((weight || dweight) && w_type != kF32 && w_type != s_type)
-        return fail(BVML_FFN_ETYPE, op + ": the weight must be f32 or of s's type");
-    const Array ady{"dy", dy, lddy, rows, cols, dy_type}, as{"s", s, lds, rows, cols, s_type};
-    const Array aw{"weight", weight, cols, 1, cols, w_type};
-    const Array ar{"rstd", rstd, rows, 1, rows, kF32};
-    const Array adst{"dstream", dstream, lddst, rows, cols, s_type};
-    const Array ads{"ds", ds, ldds, rows, cols, s_type};
-    const Array adw{"dweight", dweight, cols, 1, cols, w_type};
-    BVML_FFN_TRY(check_array(op, ady, false));
-    BVML_FFN_TRY(check_array(op, as, false));
-    if (rows > 0 && rstd == nullptr) return fail(BVML_FFN_ENULL, op + ": rstd is NULL");
-    BVML_FFN_TRY(check_array(op, adst, true));
-    BVML_FFN_TRY(check_array(op, ads, false));
-    BVML_FFN_TRY(check_alias(op, {ads, adw}, {ady, as, aw, ar, adst}, "ds", {"dstream"}));
-    const long long need = dweight ? norm_grad_workspace(rows, cols) : 0;
-    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-        return fail(BVML_FFN_EWORK, op + ": the workspace must hold " + std::to_string(need) +
-                                        " bytes");
-    const Array awork{"the workspace", workspace, need, need > 0, need, kE4M3};
-    BVML_FFN_TRY(check_alias(op, {awork}, {ady, as, aw, ar, adst, ads, adw}, nullptr, {}));
-    const NormGradCall c{dy, s, weight, rstd, dstream, lddy, lds, lddst, ldds, rows, cols, dy_type,
-                         s_type, w_type, ds, dweight, static_cast<float*>(workspace)};
-    return launched(op, launch_norm_grad(c, static_cast<hipStream_t>(stream)));
+    return guarded([&]() -> int {
+        const std::string op = "add_rms_norm_backward";
+        if (rows < 0 || cols < 1)
+            return fail(BVML_FFN_ESHAPE, op + ": rows must be >= 0, cols >= 1");
+        if (cols > kMostNormCols) return fail(BVML_FFN_ESIZE, op + ": more than 32768 columns");
+        if (rows > kMostRows) return fail(BVML_FFN_ESIZE, op + ": too many rows");
+        if (!is_value(s_type) || !is_value(dy_type))
+            return fail(BVML_FFN_ETYPE, op + ": s and dy must be f32, f16 or bf16");
+        if ((weight || dweight) && w_type != kF32 && w_type != s_type)
+            return fail(BVML_FFN_ETYPE, op + ": the weight must be f32 or of s's type");
+        const Array ady{"dy", dy, lddy, rows, cols, dy_type}, as{"s", s, lds, rows, cols, s_type};
+        const Array aw{"weight", weight, cols, 1, cols, w_type};
+        const Array ar{"rstd", rstd, rows, 1, rows, kF32};
+        const Array adst{"dstream", dstream, lddst, rows, cols, s_type};
+        const Array ads{"ds", ds, ldds, rows, cols, s_type};
+        const Array adw{"dweight", dweight, cols, 1, cols, w_type};
+        BVML_FFN_TRY(check_array(op, ady, false));
+        BVML_FFN_TRY(check_array(op, as, false));
+        if (rows > 0 && rstd == nullptr) return fail(BVML_FFN_ENULL, op + ": rstd is NULL");
+        BVML_FFN_TRY(check_array(op, adst, true));
+        BVML_FFN_TRY(check_array(op, ads, false));
+        BVML_FFN_TRY(check_alias(op, {ads, adw}, {ady, as, aw, ar, adst}, "ds", {"dstream"}));
+        const long long need = dweight ? norm_grad_workspace(rows, cols) : 0;
+        if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+            return fail(BVML_FFN_EWORK, op + ": the workspace must hold " + std::to_string(need) +
+                                            " bytes");
+        const Array awork{"the workspace", workspace, need, need > 0, need, kE4M3};
+        BVML_FFN_TRY(check_alias(op, {awork}, {ady, as, aw, ar, adst, ads, adw}, nullptr, {}));
+        const NormGradCall c{dy, s, weight, rstd, dstream, lddy, lds, lddst, ldds, rows, cols,
+                             dy_type, s_type, w_type, ds, dweight, static_cast<float*>(workspace)};
+        return launched(op, launch_norm_grad(c, static_cast<hipStream_t>(stream)));
+    });
 }
 
 int bvml_ffn_linear(const void* x, long long ldx, const void* w, long long ldw, const void* bias,
@@ -350,9 +370,11 @@ int bvml_ffn_linear(const void* x, long long ldx, const void* w, long long ldw, 
                     long long ldr, int M, int N, int K, int in_type, int out_type, int bias_type,
                     int act, void* y, long long ldy, void* z, long long ldz, void* workspace,
                     long long workspace_bytes, void* stream) {
-    return forward("linear", false, x, ldx, w, ldw, bias, x_scale, w_scale, residual, ldr, M, N, K,
-                   in_type, out_type, bias_type, act, y, ldy, z, ldz, workspace, workspace_bytes,
-                   stream);
+    return guarded([&]() -> int {
+        return forward("linear", false, x, ldx, w, ldw, bias, x_scale, w_scale, residual, ldr, M,
+                       N, K, in_type, out_type, bias_type, act, y, ldy, z, ldz, workspace,
+                       workspace_bytes, stream);
+    });
 }
 
 long long bvml_ffn_linear_workspace(int M, int N, int K, int in_type) {
@@ -364,9 +386,11 @@ int bvml_ffn_gated(const void* x, long long ldx, const void* w, long long ldw, c
                    const float* x_scale, const float* w_scale, int M, int N, int K, int in_type,
                    int out_type, int bias_type, int act, void* h, long long ldh, void* z,
                    long long ldz, void* workspace, long long workspace_bytes, void* stream) {
-    return forward("gated", true, x, ldx, w, ldw, bias, x_scale, w_scale, nullptr, 0, M, N, K,
-                   in_type, out_type, bias_type, act, h, ldh, z, ldz, workspace, workspace_bytes,
-                   stream);
+    return guarded([&]() -> int {
+        return forward("gated", true, x, ldx, w, ldw, bias, x_scale, w_scale, nullptr, 0, M, N, K,
+                       in_type, out_type, bias_type, act, h, ldh, z, ldz, workspace,
+                       workspace_bytes, stream);
+    });
 }
 
 long long bvml_ffn_gated_workspace(int M, int N, int K, int in_type) {
@@ -379,8 +403,10 @@ int bvml_ffn_linear_backward(const void* dy, long long lddy, const void* x, long
                              int N, int K, int type, int dy_type, int act, void* dx,
                              long long lddx, void* dw, long long lddw, void* db, void* workspace,
                              long long workspace_bytes, void* stream) {
-    return backward("linear_backward", false, dy, lddy, x, ldx, w, ldw, z, ldz, M, N, K, type,
-                    dy_type, act, dx, lddx, dw, lddw, db, workspace, workspace_bytes, stream);
+    return guarded([&]() -> int {
+        return backward("linear_backward", false, dy, lddy, x, ldx, w, ldw, z, ldz, M, N, K, type,
+                        dy_type, act, dx, lddx, dw, lddw, db, workspace, workspace_bytes, stream);
+    });
 }
 
 long long bvml_ffn_linear_backward_workspace(int M, int N, int K) {
@@ -393,8 +419,10 @@ int bvml_ffn_gated_backward(const void* dh, long long lddh, const void* x, long 
                             int N, int K, int type, int dh_type, int act, void* dx,
                             long long lddx, void* dw, long long lddw, void* db, void* workspace,
                             long long workspace_bytes, void* stream) {
-    return backward("gated_backward", true, dh, lddh, x, ldx, w, ldw, z, ldz, M, N, K, type,
-                    dh_type, act, dx, lddx, dw, lddw, db, workspace, workspace_bytes, stream);
+    return guarded([&]() -> int {
+        return backward("gated_backward", true, dh, lddh, x, ldx, w, ldw, z, ldz, M, N, K, type,
+                        dh_type, act, dx, lddx, dw, lddw, db, workspace, workspace_bytes, stream);
+    });
 }
 
 long long bvml_ffn_gated_backward_workspace(int M, int N, int K) {
@@ -404,25 +432,27 @@ long long bvml_ffn_gated_backward_workspace(int M, int N, int K) {
 
 int bvml_ffn_plan(int M, int R, int K, int in_type, int layout, int gated, int aligned, int* tile,
                   int* deep, int* whole, int* splits) {
-    if (M < 1 || R < 1 || K < 1)
-        return fail(BVML_FFN_ESHAPE, "plan: sizes must be >= 1");
-    if ((in_type != kE4M3 && !is16(in_type)) || layout < kForward || layout > kWeightGrad + 1 ||
-        (layout != kForward && (gated || in_type == kE4M3)))
-        return fail(BVML_FFN_ETYPE, "plan: no such product");
-    ProductPlan p;
-    if (layout <= kWeightGrad) {
-        p = plan_product(M, R, K, in_type, layout, gated != 0, aligned != 0);
-    } else {
-        const GradientsPlan g = plan_gradients(M, R, K);
-        p = {g.tile, true, g.input_splits > 1 ? g.input_whole : g.weight_whole,
-             g.input_splits > 1 ? g.input_splits : g.weight_splits};
-    }
-    static const int kRows[] = {256, 128, 128, 64, 64, 0};  // by Tile
-    if (tile) *tile = kRows[p.tile];
-    if (deep) *deep = p.tile == kTile128Deep || p.tile == kTileSquare;
-    if (whole) *whole = p.whole;
-    if (splits) *splits = p.splits;
-    return BVML_FFN_OK;
+    return guarded([&]() -> int {
+        if (M < 1 || R < 1 || K < 1)
+            return fail(BVML_FFN_ESHAPE, "plan: sizes must be >= 1");
+        if ((in_type != kE4M3 && !is16(in_type)) || layout < kForward || layout > kWeightGrad + 1 ||
+            (layout != kForward && (gated || in_type == kE4M3)))
+            return fail(BVML_FFN_ETYPE, "plan: no such product");
+        ProductPlan p;
+        if (layout <= kWeightGrad) {
+            p = plan_product(M, R, K, in_type, layout, gated != 0, aligned != 0);
+        } else {
+            const GradientsPlan g = plan_gradients(M, R, K);
+            p = {g.tile, true, g.input_splits > 1 ? g.input_whole : g.weight_whole,
+                 g.input_splits > 1 ? g.input_splits : g.weight_splits};
+        }
+        static const int kRows[] = {256, 128, 128, 64, 64, 0};  // by Tile
+        if (tile) *tile = kRows[p.tile];
+        if (deep) *deep = p.tile == kTile128Deep || p.tile == kTileSquare;
+        if (whole) *whole = p.whole;
+        if (splits) *splits = p.splits;
+        return BVML_FFN_OK;
+    });
 }
 
 const char* bvml_ffn_last_error(void) { return bvml::last_error(); }

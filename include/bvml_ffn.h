@@ -25,7 +25,8 @@
  *
  * Return value: 0 on success; a negative BVML_FFN_E* code for a rejected
  * argument (nothing is launched); a positive hipError_t value when the HIP
- * runtime reports an error at launch.  bvml_ffn_last_error() returns the
+ * runtime reports an error at launch, or hipErrorOutOfMemory when the host has
+ * no memory for a message.  bvml_ffn_last_error() returns the
  * calling thread's message for the last non-zero status.
  */
 #ifndef BVML_FFN_H
