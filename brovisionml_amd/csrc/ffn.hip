@@ -293,8 +293,8 @@ int bvml_ffn_add_rms_norm(const void* x, long long ldx, const void* residual, lo
             return fail(BVML_FFN_ESHAPE, op + ": rows must be >= 0, cols >= 1");
         if (cols > kMostNormCols) return fail(BVML_FFN_ESIZE, op + ": more than 32768 columns");
         if (rows > kMostRows) return fail(BVML_FFN_ESIZE, op + ": too many rows");
-        if (!(eps >= 0.0) || !std::isfinite(eps))
-            return fail(BVML_FFN_EPARAM, op + ": eps must be finite and >= 0");
+        if (!(eps >= 0.0) || !std::isfinite((float)eps))
+            return fail(BVML_FFN_EPARAM, op + ": eps must be >= 0 and finite in fp32");
         if (!is_value(x_type)) return fail(BVML_FFN_ETYPE, op + ": x must be f32, f16 or bf16");
         if (weight && w_type != kF32 && w_type != x_type)
             return fail(BVML_FFN_ETYPE, op + ": the weight must be f32 or of x's type");

@@ -42,7 +42,7 @@ extern "C" {
 #define BVML_FFN_ETYPE (-3)   /* a type or a mixture of types the operator does not take */
 #define BVML_FFN_ESIZE (-4)   /* a size beyond the kernels' index range */
 #define BVML_FFN_EALIAS (-5)  /* an output or the workspace overlaps another argument */
-#define BVML_FFN_EPARAM (-6)  /* eps negative or not finite, an unknown activation */
+#define BVML_FFN_EPARAM (-6)  /* eps negative or not finite in fp32, an unknown activation */
 #define BVML_FFN_EWORK (-7)   /* the workspace is missing, too small or not on 16 bytes */
 
 /* Element types. */

@@ -119,3 +119,10 @@ def test_no_rows_in_any_dimension(shape):
     assert ffn._rows("op", "x", t)[:2] == (0, 64)
     wide = torch.zeros(*shape[:-1], 100)[..., :64]
     assert ffn._rows("op", "x", wide)[:2] == (0, 64)
+
+
+@pytest.mark.parametrize("eps", [1e39, 1e308, float("inf")])
+def test_norm_refuses_an_eps_that_fp32_does_not_hold(eps):
+    # (no rows: nothing could be launched)
+    assert norm(rows=0, eps=eps) == _lib.FFN_EPARAM
+    assert norm(rows=0, eps=3e38) == _lib.OK
