@@ -10,7 +10,7 @@
 // sums are fp32.  A team is a workgroup of a wave for every 512 columns; rows
 // of one wave share a workgroup of four (BVML_FFN_TEAMS below, with the times).
 //
-// 4805 x 1280 from fp32 to 8 bits, the sum stored too: 14.6 us, 5.5 TB/s.  The
+// 4805 x 1280 from fp32 to 8 bits, the sum stored too: 14.7 us, 5.4 TB/s.  The
 // gradient of 65541 x 1024: 119 us, 4.5 TB/s, with 5 of them the weight's sums.
 
 #include "ffn_kernels.h"

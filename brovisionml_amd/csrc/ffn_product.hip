@@ -354,7 +354,8 @@ hipError_t launch_rows_of(const Product& a, bool whole, hipStream_t s) {
         // from 3 rows on, once two workgroups a CU are left: 4 x 1280 x 8192 7.3
         // to 6.3 us; 1 x 1280 x 5120 takes 4.3 either way, and 4 x 5120 x 2048 7.3
         // for 6.5.  Gated waves have two columns as it is: four take 4 x 1280 x 5120
-        // from 7.3 to 7.6.
+        // from 7.3 to 7.6 (all with the weights in the caches; from memory the
+        // latter takes 10.5).
         if constexpr (!kGated) {
             if (a.e.N >= 4096) return launch_dot_one<kIn, 4, 2, kGated>(a, whole, s);
         }
@@ -390,7 +391,8 @@ bool dma_fits(const ProductCall& c) {
 
 namespace {
 
-// What a tile costs, in us, measured on bf16 products of 1,280 to 8,192 terms:
+// What a tile costs, in us, measured on bf16 products of 1,280 to 8,192 terms
+// (8-bit ones are chosen by the same figures):
 // `fixed` for its first copies and its epilogue, `step` for 128 bytes of k with
 // the card full and `idle` with half of that at most.
 // `room`: workgroups on the card at once, one or two a CU.

@@ -450,7 +450,9 @@ def linear_backward(dy, x, w, z=None, act: str = "none", *, need_x: bool = True,
                     need_w: bool = True, need_bias: bool = True):
     """(dx, dw, dbias) of linear, in x's type, from dy (x's type or float32),
     its inputs and its saved z (not needed with act "none"); None for those
-    not needed.  The residual's gradient is dy itself."""
+    not needed.  The residual's gradient is dy itself.  The products take
+    dz = dy act'(z) in x's type: with float16 a float32 dy, too, is cut to its
+    range."""
     return _backward("linear_backward", False, dy, x, w, z, act, need_x, need_w, need_bias)
 
 

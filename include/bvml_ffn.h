@@ -6,13 +6,13 @@
  *   linear         y = act(x W^T + b) + r
  *   gated          h = act(x Wg^T + bg) * (x Wu^T + bu),  W = [Wg; Wu]
  *
- * For the transformer encoders that run beside the DSINE path.  The reference
- * composes such blocks from brotensor ops; these fused forms have no
- * counterpart in it.
+ * For transformer blocks that a program runs beside the DSINE path, which uses
+ * none of them.  The reference composes such blocks from brotensor ops; these
+ * fused forms have no counterpart in it.
  *
  * Every matrix is row-major with its rows `ld` elements apart and the elements
- * of a row adjacent; no alignment is required (16-byte aligned rows take the
- * fastest kernels).  Plain pointers and scalars only: every pointer is a device
+ * of a row adjacent, at most 2^23 - 256 bytes from row to row; no alignment is
+ * required (16-byte aligned rows take the fastest kernels).  Plain pointers and scalars only: every pointer is a device
  * pointer, every call is asynchronous on `stream` (NULL = the null stream),
  * allocates nothing, keeps nothing, and nothing throws.  Calls can be captured
  * into a HIP graph.  Equal inputs give equal bits.
@@ -70,7 +70,8 @@ extern "C" {
  *               scale = max(max|y| / 448, 2^-126), q = y / scale to nearest
  *   rstd        (rows) fp32, or NULL: kept for the backward pass
  * A row with a NaN or an infinity in s has NaN where the formula has; in E4M3
- * its scale is NaN or infinite with it.  y is formed from the unrounded s.
+ * its scale is NaN or infinite with it.  y is formed from the unrounded s.  The
+ * mean of squares is fp32's: a finite s beyond 1.8e19 makes rstd, and y, 0.
  */
 int bvml_ffn_add_rms_norm(const void* x, long long ldx, const void* residual, long long ldr,
                           const void* weight, int rows, int cols, double eps, int x_type,
@@ -124,7 +125,8 @@ long long bvml_ffn_gated_workspace(int M, int N, int K, int in_type);
  * dz = dy act'(z) rounded to `type` for the products,
  *   dx = dz W (M, K);  dw = dz^T x (N, K);  db = sum over rows of dz (N).
  * Any of the three may be NULL.  dy is of dy_type (`type` or F32); z may be
- * NULL with act NONE.  The residual's gradient is dy itself.
+ * NULL with act NONE.  The residual's gradient is dy itself.  With F16 dz ends
+ * at 65504 and below 2^-25 it is 0, from an F32 dy too: scale the loss for it.
  */
 int bvml_ffn_linear_backward(const void* dy, long long lddy, const void* x, long long ldx,
                              const void* w, long long ldw, const void* z, long long ldz, int M,
